@@ -88,8 +88,8 @@ int pdes_context_device(const pdes_context* ctx);
 /* ABI version of this header; bumped on any signature change. */
 int pdes_abi_version(void);
 /* sizeof of a boundary structure: 0 pdes_conv_desc, 1 pdes_pack_item, 2 pdes_mfma_pack_item, 3 pdes_up_pack_item,
- * 4 pdes_b3_pack_item, 5 pdes_b3up_pack_item, 6 pdes_reduce_item, 7 pdes_bn_item, 8 pdes_op; -1 otherwise (a binding checks
- * its own mirrors against it) */
+ * 4 pdes_b3_pack_item, 5 pdes_b3up_pack_item, 6 pdes_reduce_item, 7 pdes_bn_item, 8 pdes_op, 9 pdes_mt_tensor,
+ * 10 pdes_adamw_class, 11 pdes_adamw_state; -1 otherwise (a binding checks its own mirrors against it) */
 int pdes_sizeof(int which);
 /* number of replicas of the fp64 accumulator arena the kernels are compiled for (see pdes_conv_desc.nrep) */
 int pdes_stat_replicas(void);
@@ -583,6 +583,61 @@ int pdes_mse_loss(const float* output, const float* target, float* grad_out, dou
  * solve_conv_mixed_residual.py:124) on the Gram matrix of the history. */
 int pdes_multi_dot(const float* W, long long ld, int rows, const float* V, int nv, long long n, double* partials,
                    int nsplit, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Operators over a LIST of tensors (no reference counterpart; torch.optim.AdamW and torch.nn.utils.clip_grad_norm_ are the
+ * interfaces behind which pde_surrogate_amd/adamw.py puts them).  `params`, `grads`: host arrays of device addresses, aligned
+ * to the element only, each tensor dense; everything that describes the list is read at call time and passed to the kernels by
+ * value.  Lists of any length (a launch takes 96 or 160 tensors), tensors of 0 to 2^40 - 1 elements.  All tensors of a call
+ * have one element type; several calls make a mixed list. */
+enum { PDES_MT_F32 = 0, PDES_MT_BF16 = 1, PDES_MT_F16 = 2 };
+#define PDES_MT_BLOCK 256    /* elements that share a scale of 8-bit states; every tensor's state starts at a multiple */
+#define PDES_MT_CLASSES 8    /* hyper-parameter sets of one pdes_adamw_step call */
+#define PDES_MT_ROWS 256     /* doubles that pdes_grad_norm writes */
+#define PDES_MT_HYPER_BYTES 288  /* bytes of pdes_adamw_state.hyper */
+
+/* Partial results of the norm of a list into rows[PDES_MT_ROWS]: kind 2 sums of squares (fp64, fixed order: the same list gives
+ * the same bits), kind 0 largest magnitudes (NaN if any element is NaN).  add != 0: on top of what rows hold. */
+int pdes_grad_norm(const unsigned long long* grads, const long long* sizes, int count, int dtype, int kind, double* rows,
+                   int add, void* stream);
+/* norm_out[0] (nullable, fp32) = the norm that `rows` make, and grads *= min(1, limit / (norm + 1e-6)) in place; limit =
+ * infinity finds the norm only; a factor of 1 writes nothing.  limit < 0 or NaN: PDES_EINVAL. */
+int pdes_clip_grads(const unsigned long long* grads, const long long* sizes, int count, int dtype, int kind,
+                    const double* rows, float limit, float* norm_out, void* stream);
+
+typedef struct pdes_mt_tensor {
+  long long n;       /* elements */
+  long long block0;  /* first block of its state: element index PDES_MT_BLOCK * block0 of the state buffers */
+  int cls;           /* its entry of `classes` */
+  int ordinal;       /* its number in the random sequence of the 8-bit states (its place in the optimiser) */
+} pdes_mt_tensor;
+typedef struct pdes_adamw_class {
+  double lr, beta1, beta2, eps, weight_decay;
+  long long step;         /* number of this step, from 1 (ignored when step_dev is given) */
+  float* step_dev;        /* device step count, incremented by the call: all classes of a call or none */
+  const float* lr_dev;    /* with step_dev: learning rate read from the device instead of lr (nullable) */
+} pdes_adamw_class;
+typedef struct pdes_adamw_state {
+  void* exp_avg;          /* bits 32: fp32; bits 8: e4m3 codes.  PDES_MT_BLOCK * blocks elements, 16-byte aligned */
+  void* exp_avg_sq;       /* bits 32: fp32 second moments; bits 8: e4m3 codes of their square roots */
+  float* exp_avg_scale;   /* bits 8: one per block */
+  float* rms_scale;       /* bits 8: one per block */
+  short* low;             /* bf16 parameters: the 16 bits below each (nullable: parameters are rounded to nearest) */
+  long long blocks;       /* blocks that the state buffers hold */
+  const double* norm_rows;/* of pdes_grad_norm: gradients are multiplied by min(1, limit / (norm + 1e-6)) as they are read */
+  float* norm_out;        /* with norm_rows: the norm (nullable) */
+  void* hyper;            /* with step_dev: PDES_MT_HYPER_BYTES of device scratch */
+  float limit;
+  int dtype, bits, maximize;
+  unsigned seed;          /* bits 8: of the stochastic rounding */
+} pdes_adamw_state;
+/* One AdamW step (decoupled weight decay, bias correction, eps outside the root):
+ *   g = factor * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32, one rounding per operation; gradients are left as they are.  The elements of the state buffers behind a tensor's
+ * last element, up to its block's end, stay zero if they were. */
+int pdes_adamw_step(const unsigned long long* params, const unsigned long long* grads, const pdes_mt_tensor* tensors,
+                    int count, const pdes_adamw_class* classes, int nclasses, const pdes_adamw_state* state, void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,7 +5,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libpdes_hip.so')
-ABI_VERSION = 24
+ABI_VERSION = 25
 
 _c_f = ctypes.c_float
 _c_i = ctypes.c_int
@@ -60,6 +60,9 @@ SIGNATURES = {
     'pdes_adam_step': [_c_p, _c_p, _c_p, _c_p, _c_p, _c_f, ctypes.c_longlong, _c_p],
     'pdes_adam_step_host': [_c_p, _c_p, _c_p, _c_p, _c_p, _c_f, _c_i, ctypes.c_longlong, _c_p],
     'pdes_adam_step_host2': [_c_p, _c_p, _c_p, _c_p, _c_p, _c_f, _c_i, ctypes.c_longlong, _c_p, ctypes.c_longlong, _c_p],
+    'pdes_grad_norm': [_c_p, _c_p, _c_i, _c_i, _c_i, _c_p, _c_i, _c_p],
+    'pdes_clip_grads': [_c_p, _c_p, _c_i, _c_i, _c_i, _c_p, _c_f, _c_p, _c_p],
+    'pdes_adamw_step': [_c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_p],
     'pdes_test_metrics': [_c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_p],
     'pdes_mse_partials': [ctypes.c_longlong],
     'pdes_mse_loss': [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, ctypes.c_longlong, _c_p],

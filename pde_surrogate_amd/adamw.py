@@ -1,0 +1,482 @@
+"""AdamW over many tensors at once, and clipping by the gradients' common norm.
+
+    opt = optim.FusedAdamW(model.parameters(), lr=1e-3, weight_decay=0.01)                 # 32-bit states
+    opt = optim.FusedAdamW(model.parameters(), lr=1e-3, state_bits=8, clip_norm=1.0)       # 8-bit states, clipped
+    norm = optim.clip_grad_norm_(model.parameters(), 1.0)                                  # for any optimiser
+
+Any list of fp32, bf16 or fp16 parameters on one GPU takes part, whichever module they belong to: `optim.Adam` needs one HIP
+network's flat buffer for its one-launch step, `FusedAdamW` takes the tensors as they are, up to 96 in a launch.  The
+kernels are csrc/multi_tensor.hip; the arithmetic is fp32 with one rounding per operation (include/pdes_hip.h:
+pdes_adamw_step), the norm's sum is fp64 in a fixed order, so equal inputs give equal bits.
+"""
+import ctypes
+import math
+from array import array
+from collections import defaultdict
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                   # PDES_MT_BLOCK: every tensor's state starts at a multiple of it; elements that share a scale
+_CLASSES = 8                  # PDES_MT_CLASSES
+_ROWS = 256                   # PDES_MT_ROWS
+_HYPER_BYTES = 288            # PDES_MT_HYPER_BYTES
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class MtTensor(ctypes.Structure):
+    _fields_ = [('n', ctypes.c_longlong), ('block0', ctypes.c_longlong), ('cls', ctypes.c_int), ('ordinal', ctypes.c_int)]
+
+
+class AdamWClass(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_double) for k in ('lr', 'beta1', 'beta2', 'eps', 'weight_decay')] + \
+               [('step', ctypes.c_longlong), ('step_dev', ctypes.c_void_p), ('lr_dev', ctypes.c_void_p)]
+
+
+class AdamWState(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ('exp_avg', 'exp_avg_sq', 'exp_avg_scale', 'rms_scale', 'low')] + \
+               [('blocks', ctypes.c_longlong), ('norm_rows', ctypes.c_void_p), ('norm_out', ctypes.c_void_p),
+                ('hyper', ctypes.c_void_p), ('limit', ctypes.c_float), ('dtype', ctypes.c_int), ('bits', ctypes.c_int),
+                ('maximize', ctypes.c_int), ('seed', ctypes.c_uint)]
+
+
+_data_ptr = torch.Tensor.data_ptr
+_get_device = torch.Tensor.get_device
+_numel = torch.Tensor.numel
+_is_contiguous = torch.Tensor.is_contiguous
+
+
+def _dense(t):
+    """whether the elements of `t` fill one stretch of memory, each once (any order of the dimensions)"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_order(a, b):
+    """whether element k of a's memory is element k of b's"""
+    return all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
+def _check_tensor(t, what):
+    if t.layout != torch.strided:
+        raise RuntimeError(f'{what}: sparse tensors are not supported')
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f'{what}: expected float32, bfloat16 or float16, got {t.dtype}')
+    if not t.is_cuda:
+        raise RuntimeError(f'pde_surrogate_amd runs on an MI355X only: {what} is a CPU tensor (there is no CPU fallback; '
+                           'move tensors to cuda)')
+
+
+def _addresses(tensors):
+    return array('Q', map(_data_ptr, tensors))
+
+
+def _repeated(pairs):
+    """whether one of the (address, size) pairs with elements appears twice"""
+    used = [x for x, n in pairs if n]
+    return len(set(used)) < len(used)
+
+
+def _norm_rows(lists, kind, device):
+    """pdes_grad_norm over [(element type, addresses, sizes)]: the rows, on the current stream"""
+    rows = torch.empty(_ROWS, dtype=torch.float64, device=device)
+    stream = _lib.stream_ptr(device)
+    for k, (dtype, ptrs, sizes) in enumerate(lists):
+        rc = _lib.lib().pdes_grad_norm(ptrs.buffer_info()[0], sizes.buffer_info()[0], len(ptrs), dtype, kind, rows.data_ptr(),
+                                       int(k > 0), stream)
+        _lib.check(rc, 'pdes_grad_norm')
+    return rows
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ for parameters on one GPU: returns the norm of all gradients taken as one vector (0-d
+    fp32 on the device) and multiplies the gradients in place by min(1, max_norm / (norm + 1e-6)), without synchronising.
+    norm_type is 2 (summed in fp64) or infinity.  max_norm = inf finds the norm only.  Where the factor is 1 the gradients
+    are read once and not written.  A gradient that is not dense (an expanded one) or appears twice is refused.
+    error_if_nonfinite waits for the norm and raises, with the gradients as they were, if it is not finite."""
+    grads = [p.grad for p in ([parameters] if isinstance(parameters, torch.Tensor) else parameters) if p.grad is not None]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f'clip_grad_norm_: norm_type {norm_type} is not supported (2 or inf)')
+    if not max_norm >= 0.0:
+        raise ValueError(f'clip_grad_norm_: max_norm {max_norm} must not be negative')
+    if not grads:
+        return torch.tensor(0.0)
+    by_type = {}
+    for g in grads:
+        _check_tensor(g, 'a gradient')
+        if not _dense(g):
+            raise RuntimeError('clip_grad_norm_: a gradient is not dense')
+        by_type.setdefault(g.dtype, []).append(g)
+    if len(set(map(_get_device, grads))) > 1:
+        raise RuntimeError(f'clip_grad_norm_: gradients on several devices ({sorted(set(map(_get_device, grads)))})')
+    lists = [(_DTYPES[t], _addresses(gs), array('q', map(_numel, gs))) for t, gs in by_type.items()]
+    if _repeated((x, n) for _, ptrs, sizes in lists for x, n in zip(ptrs, sizes)):
+        raise ValueError('clip_grad_norm_: a gradient appears twice')
+    device = grads[0].device
+    kind = 2 if norm_type == 2.0 else 0
+
+    def clip(dtype, ptrs, sizes, limit, norm):
+        rc = _lib.lib().pdes_clip_grads(ptrs.buffer_info()[0], sizes.buffer_info()[0], len(ptrs), dtype, kind, rows.data_ptr(), limit,
+                                        norm.data_ptr(), _lib.stream_ptr(device))
+        _lib.check(rc, 'pdes_clip_grads')
+
+    with _lib.device_guard(device):
+        rows = _norm_rows(lists, kind, device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        if error_if_nonfinite or max_norm == math.inf:
+            clip(*lists[0], math.inf, norm)
+            if error_if_nonfinite and not math.isfinite(float(norm)):
+                raise RuntimeError(f'the norm of order {norm_type} of the gradients is not finite, so they cannot be clipped; with '
+                                   'error_if_nonfinite=False they are multiplied by the factor that it gives')
+        if max_norm != math.inf:
+            for x in lists:
+                clip(*x, max_norm, norm)
+            torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+class _Arena:
+    """state buffers of a list of parameters of one element type, each from a multiple of BLOCK elements on"""
+
+    def __init__(self, dtype, blocks, bits, master, device):
+        self.dtype, self.blocks = dtype, blocks
+
+        def zeros(n, t):
+            return torch.zeros(n, dtype=t, device=device)
+        n = blocks * BLOCK
+        if bits == 32:
+            self.bufs = {'exp_avg': zeros(n, torch.float32), 'exp_avg_sq': zeros(n, torch.float32)}
+        else:
+            self.bufs = {'exp_avg_q': zeros(n, torch.uint8).view(torch.float8_e4m3fn), 'exp_avg_scale': zeros(blocks, torch.float32),
+                         'rms_q': zeros(n, torch.uint8).view(torch.float8_e4m3fn), 'rms_scale': zeros(blocks, torch.float32)}
+        if master and dtype == torch.bfloat16:
+            self.bufs['low'] = zeros(n, torch.int16)
+        self.stream = torch.cuda.current_stream(device)
+
+    def views(self, p, block0):
+        """{name: the part of it that belongs to p}: in p's shape and order where there is one value per element"""
+        n, blocks = p.numel(), -(-p.numel() // BLOCK)
+        out = {}
+        for name, buf in self.bufs.items():
+            if name.endswith('_scale'):
+                out[name] = buf[block0:block0 + blocks]
+            elif name.endswith('_q'):
+                out[name] = buf[block0 * BLOCK:(block0 + blocks) * BLOCK]
+            else:
+                out[name] = buf.as_strided(p.shape, p.stride(), block0 * BLOCK) if n else buf[:0].view(p.shape)
+        return out
+
+
+class _Launch:
+    """one pdes_adamw_step call: parameters of one arena in up to eight classes"""
+
+    def __init__(self, arena, members, classes):
+        # members: (parameter, its class, block0, ordinal); classes: (param_group, step tensor)
+        self.arena, self.classes = arena, classes
+        self.params = [m[0] for m in members]
+        self.sizes = array('q', (p.numel() for p in self.params))
+        self.size_list = list(self.sizes)
+        self.tensors = (MtTensor * len(members))(*[MtTensor(p.numel(), b, c, o) for p, c, b, o in members])
+        self.table = (AdamWClass * len(classes))()
+        self.state = AdamWState()
+        for name, key in (('exp_avg', 'exp_avg'), ('exp_avg_sq', 'exp_avg_sq'), ('exp_avg', 'exp_avg_q'), ('exp_avg_sq', 'rms_q'),
+                          ('exp_avg_scale', 'exp_avg_scale'), ('rms_scale', 'rms_scale'), ('low', 'low')):
+            if key in arena.bufs:
+                setattr(self.state, name, arena.bufs[key].data_ptr())
+        self.state.blocks, self.state.dtype = arena.blocks, _DTYPES[arena.dtype]
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay, torch.optim.AdamW's update) over any fp32 / bf16 / fp16 parameters of one GPU.
+
+    state_bits      32: exp_avg and exp_avg_sq in fp32, in the parameter's shape: a torch.optim.AdamW state_dict loads here and
+                    the other way round.  8: both moments in 8 bits (e4m3, the second one as its square root) with an fp32
+                    scale for each 256 elements and stochastic rounding: 2.06 bytes per element instead of 8.
+    master_weights  bf16 parameters keep the 16 bits that bf16 cuts off (state 'low', 2 bytes per element), so that the step
+                    works on fp32 weights; a parameter that the program overwrites is taken as it is, to half of its last
+                    place.  Without it a bf16 / fp16 parameter is rounded to nearest after every step, as torch does.
+    clip_norm       gradients are multiplied by min(1, clip_norm / (norm + 1e-6)) as the step reads them, the norm taken over
+                    all gradients of the step; `.grad` stays as it is, `grad_norm` is the norm (0-d tensor on the device).
+    capturable      step counts live on the device (and `lr` may be a 0-d device tensor), so that a step may be captured into
+                    a graph; take one eager step first, which makes the states.
+    seed            of the stochastic rounding: equal seeds, parameters and gradients give equal bits.
+
+    A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
+    dense.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse and complex parameters are
+    not offered.  A gradient that is not finite spoils the elements it belongs to and no others."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
+                 clip_norm=None, maximize=False, capturable=False, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits {state_bits} is not supported (8 or 32)')
+        if clip_norm is not None and not float(clip_norm) >= 0.0:
+            raise ValueError(f'clip_norm {clip_norm} must not be negative')
+        if not 0 <= int(seed) < 1 << 32:
+            raise ValueError(f'seed {seed} is not in [0, 2^32)')
+        self.state_bits, self.master_weights, self.maximize = state_bits, bool(master_weights), bool(maximize)
+        self.clip_norm, self.capturable, self.seed = None if clip_norm is None else float(clip_norm), bool(capturable), int(seed)
+        self.grad_norm = None
+        self._retired = []
+        self._reset()
+        self._device = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _reset(self):
+        self._where = {}            # parameter -> (arena, block0)
+        self._arenas = []
+        self._plan = None           # (which parameters have gradients, [_Launch], the state dictionary, its length)
+
+    def _retire(self, *what):
+        """a captured graph may still write to buffers that have been replaced: they stay until the optimiser goes"""
+        if self.capturable:
+            self._retired.extend(what)
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        try:
+            self._check_group(group)
+        except Exception:
+            self.param_groups.pop()
+            raise
+        self._plan = None
+
+    def _check_group(self, group):
+        device = self._device
+        lr, (b1, b2) = group['lr'], group['betas']
+        if isinstance(lr, torch.Tensor) and not (self.capturable and lr.is_cuda and lr.dim() == 0 and lr.dtype == torch.float32):
+            raise ValueError('lr as a tensor has to be a 0-d float32 device tensor of an optimiser with capturable=True')
+        if not isinstance(lr, torch.Tensor) and not 0.0 <= lr:
+            raise ValueError(f'Invalid learning rate: {lr}')
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f'Invalid betas: {group["betas"]}')
+        if not 0.0 <= group['eps']:
+            raise ValueError(f'Invalid epsilon value: {group["eps"]}')
+        if not 0.0 <= group['weight_decay']:
+            raise ValueError(f'Invalid weight_decay value: {group["weight_decay"]}')
+        for p in group['params']:
+            _check_tensor(p, 'a parameter')
+            if not _dense(p):
+                raise ValueError('a parameter is not dense (its elements do not fill one stretch of memory)')
+            if device is None:
+                device = p.device
+            elif p.device != device:
+                raise ValueError(f'parameters on {device} and {p.device}')
+        if len({id(p) for p in group['params']}) < len(group['params']):
+            raise ValueError('a parameter appears twice')
+        self._device = device
+
+    # -- states ----------------------------------------------------------------------------------------------------------
+    def _make_states(self, params):
+        """states of parameters that have none, or have some from elsewhere (a loaded or copied state): one arena per type"""
+        by_type = {}
+        for p in params:
+            by_type.setdefault(p.dtype, []).append(p)
+        for dtype, ps in by_type.items():
+            arena = _Arena(dtype, sum(-(-p.numel() // BLOCK) for p in ps), self.state_bits, self.master_weights, self._device)
+            self._arenas.append(arena)
+            block0, fresh = 0, None
+            for p in ps:
+                mine, had = arena.views(p, block0), self.state[p]
+                if had:
+                    for name, view in mine.items():
+                        if name not in had:
+                            raise ValueError(f'the state of a parameter has no {name!r}: it comes from an optimiser with other '
+                                             f'state_bits or master_weights (it has {sorted(map(str, had))})')
+                        old = had[name]
+                        if tuple(old.shape) != tuple(view.shape):
+                            raise ValueError(f'state {name!r} has shape {tuple(old.shape)}, the parameter needs {tuple(view.shape)}')
+                        view.copy_(old)
+                    mine['step'] = self._step_tensor(float(had['step']))
+                else:
+                    fresh = self._step_tensor(0.0) if fresh is None else fresh
+                    mine['step'] = fresh
+                self.state[p] = {k: mine[k] for k in ('step', *arena.bufs)}
+                self._where[p] = (arena, block0)
+                block0 += -(-p.numel() // BLOCK)
+
+    def _step_tensor(self, value):
+        return torch.tensor(value, dtype=torch.float32, device=self._device if self.capturable else 'cpu')
+
+    def flat_state(self):
+        """{name: [the flat buffers that hold this state, one per element type]}: the parameters' states one behind the other
+        in the order of the parameter list, each from a multiple of 256 elements on ('..._scale': one value per 256)"""
+        out = {}
+        for arena in self._arenas:
+            for name, buf in arena.bufs.items():
+                out.setdefault(name, []).append(buf)
+        return out
+
+    def __getstate__(self):
+        keep = ('state_bits', 'master_weights', 'maximize', 'clip_norm', 'capturable', 'seed', '_device')
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in keep}}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.grad_norm = None
+        self._retired = []
+        self._reset()
+
+    def state_dict(self):
+        sd = super().state_dict()
+        # here parameters that are stepped together share one count; another optimiser would count it once for each of them
+        sd['state'] = {k: {**v, 'step': v['step'].clone()} if 'step' in v else v for k, v in sd['state'].items()}
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        saved, groups = state_dict['state'], state_dict['param_groups']
+        if any(g.get('amsgrad') for g in groups):
+            raise ValueError('load_state_dict: amsgrad states are not supported')
+        ours, theirs = [p for g in self.param_groups for p in g['params']], [i for g in groups for i in g['params']]
+        before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_retired', '_where', '_arenas', '_plan')}
+        steps = [st['step'] for st in self.state.values() if 'step' in st]
+        try:
+            # the base class would convert the states to their parameters' type: it gets the groups alone
+            super().load_state_dict({'state': {}, 'param_groups': groups})
+            self.state = defaultdict(dict, {p: dict(saved[i]) for i, p in zip(theirs, ours) if saved.get(i)})
+            for g in self.param_groups:
+                self._check_group(g)
+            with _lib.device_guard(self._device):
+                self._make_states(list(self.state))
+        except Exception:                  # an optimiser that cannot take the dictionary is left as it was
+            self.__dict__.update(before)
+            raise
+        self._retired = before['_retired']
+        self._retire(before['_arenas'], steps)
+
+    # -- the step --------------------------------------------------------------------------------------------------------
+    def _build(self, have):
+        """the launches of a step in which the parameters marked in `have` take part"""
+        every = [(g, p) for g in self.param_groups for p in g['params']]
+        active = [(g, p, k) for k, ((g, p), h) in enumerate(zip(every, have)) if h]
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('FusedAdamW: the first step, and the first one with gradients for other parameters than before, cannot '
+                               'be captured into a graph: take it eagerly')
+        if self._where and not any('step' in self.state.get(p, ()) for p in self._where):
+            self._retire(self._arenas)
+            self._reset()                  # the program has emptied the states, or put others in their place
+        if _repeated((p.data_ptr(), p.numel()) for _, p, _ in active):
+            raise RuntimeError('FusedAdamW: two parameters share their memory')
+        new = [p for _, p, _ in active if p not in self._where or 'step' not in self.state.get(p, ())]
+        if new:
+            self._make_states(new)
+        # a class: a group's parameters of one arena at the same step.  They share one count, which the call increments once.
+        # On the device the values are unknown: there, what has shared a count so far goes on sharing it
+        holders, classes = {}, {}
+        for p in self._where:
+            step = self.state.get(p, {}).get('step')
+            holders[id(step)] = holders.get(id(step), 0) + 1
+        for g, p, k in active:
+            (arena, block0), step = self._where[p], self.state[p]['step']
+            key = (id(arena), id(g), id(step) if self.capturable else float(step))
+            classes.setdefault(key, (arena, g, step, []))[3].append((p, block0, k))
+        counted = {}
+        for key, (arena, g, step, members) in classes.items():
+            if not (self.capturable and holders[id(step)] == len(members)):
+                self._retire(step)
+                step = step.clone()
+            for p, _, _ in members:
+                self.state[p]['step'] = step
+            counted[key] = step
+        launches = []
+        for arena in self._arenas:
+            keys = [k for k in classes if k[0] == id(arena)]
+            for at in range(0, len(keys), _CLASSES):
+                part = keys[at:at + _CLASSES]
+                members = sorted(((p, c, b, o) for c, key in enumerate(part) for p, b, o in classes[key][3]), key=lambda m: m[3])
+                launches.append(_Launch(arena, members, [(classes[key][1], counted[key]) for key in part]))
+        self._plan = (have, launches, self.state, len(self.state))
+        return launches
+
+    def _gradients(self, launch):
+        """the launch's gradients, after everything that the kernels rely on has been looked at"""
+        params = launch.params
+        grads = [p.grad for p in params]
+        dtype, device = launch.arena.dtype, self._device.index
+        try:
+            plain = all(map(_is_contiguous, params)) and all(map(_is_contiguous, grads))
+        except RuntimeError:                                    # (a sparse tensor does not say)
+            plain = False
+        if not plain:
+            for k, (p, g) in enumerate(zip(params, grads)):
+                if g.layout != torch.strided:
+                    raise RuntimeError('FusedAdamW does not support sparse gradients')
+                if not _dense(p):
+                    raise RuntimeError('FusedAdamW: a parameter is no longer dense')
+                if not (_dense(g) and _same_order(p, g)):
+                    grads[k] = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        if list(map(_numel, params)) != launch.size_list or list(map(_numel, grads)) != launch.size_list:
+            raise RuntimeError('FusedAdamW: a parameter has another size than its state')
+        for ts in (params, grads):
+            if set(map(_get_device, ts)) != {device} or any(t.dtype is not dtype for t in ts):
+                raise RuntimeError(f'FusedAdamW: a parameter or gradient is no longer a {dtype} tensor on {self._device}')
+        return grads
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        have = [p.grad is not None for g in self.param_groups for p in g['params']]
+        with _lib.device_guard(self._device):
+            if torch.cuda.is_current_stream_capturing() and not self.capturable:
+                raise RuntimeError('FusedAdamW: a step is captured into a graph only with capturable=True')
+            plan = self._plan
+            fits = plan is not None and plan[0] == have and plan[2] is self.state and plan[3] == len(self.state)
+            self._run(plan[1] if fits else self._build(have))
+        return loss
+
+    def _run(self, launches):
+        device, L = self._device, _lib.lib()
+        current = torch.cuda.current_stream(device)
+        stream = current.cuda_stream
+        grads = [self._gradients(x) for x in launches]          # (kept until the launches are enqueued)
+        ptrs = [_addresses(g) for g in grads]
+        rows = None
+        if self.clip_norm is not None:
+            if not any(map(sum, (x.sizes for x in launches))):
+                self.grad_norm = torch.zeros((), dtype=torch.float32, device=device)
+            else:
+                rows = _norm_rows([(x.state.dtype, a, x.sizes) for x, a in zip(launches, ptrs)], 2, device)
+                self.grad_norm = norm = torch.empty((), dtype=torch.float32, device=device)
+        capturing = torch.cuda.is_current_stream_capturing()
+        for x, a in zip(launches, ptrs):
+            st = x.state
+            st.bits, st.maximize, st.seed = self.state_bits, self.maximize, self.seed
+            if rows is not None:
+                st.norm_rows, st.norm_out, st.limit = rows.data_ptr(), norm.data_ptr(), self.clip_norm
+            else:
+                st.norm_rows = None
+            if self.capturable:
+                hyper = torch.empty(_HYPER_BYTES, dtype=torch.uint8, device=device)
+                st.hyper = hyper.data_ptr()
+            for c, (g, step) in zip(x.table, x.classes):
+                lr = g['lr']
+                c.beta1, c.beta2 = g['betas']
+                c.eps, c.weight_decay = g['eps'], g['weight_decay']
+                if self.capturable:
+                    c.step_dev = step.data_ptr()
+                    c.lr_dev = lr.data_ptr() if isinstance(lr, torch.Tensor) else None
+                    c.lr = 0.0 if isinstance(lr, torch.Tensor) else lr
+                else:
+                    step += 1
+                    c.step, c.lr = int(step), lr
+            where = _addresses(x.params)
+            rc = L.pdes_adamw_step(where.buffer_info()[0], a.buffer_info()[0], x.tensors, len(x.params), x.table, len(x.classes),
+                                   ctypes.byref(st), stream)
+            _lib.check(rc, 'pdes_adamw_step')
+            torch.autograd.graph.increment_version(x.params)
+            if x.arena.stream != current and not capturing:     # freed later than this stream's work on them
+                for buf in x.arena.bufs.values():
+                    buf.record_stream(current)

@@ -16,6 +16,9 @@ CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libpdes_hip.so')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-ffp-contract=fast',
          '-Wno-unused-result', '-munsafe-fp-atomics']
+# added for one source: the list operators round every product and sum once (no contraction), and use no packed fp32
+# instructions
+FILE_FLAGS = {'multi_tensor.hip': ['-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
 
 
 def sources():
@@ -45,7 +48,7 @@ def build(force=False, verbose=True):
         objs.append(obj)
         if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(
                 [os.path.getmtime(src)] + [os.path.getmtime(h) for h in headers()]):
-            cmd = [hipcc] + [f for f in FLAGS if f != '-shared'] + os.environ.get('PDES_EXTRA_FLAGS', '').split() + ['-c', src, '-o', obj]
+            cmd = [hipcc] + [f for f in FLAGS if f != '-shared'] + FILE_FLAGS.get(os.path.basename(src), []) + os.environ.get('PDES_EXTRA_FLAGS', '').split() + ['-c', src, '-o', obj]
             if verbose:
                 print(' '.join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))

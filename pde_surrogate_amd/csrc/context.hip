@@ -103,6 +103,9 @@ extern "C" int pdes_sizeof(int which) {
     case 6: return (int)sizeof(pdes_reduce_item);
     case 7: return (int)sizeof(pdes_bn_item);
     case 8: return (int)sizeof(pdes_op);
+    case 9: return (int)sizeof(pdes_mt_tensor);
+    case 10: return (int)sizeof(pdes_adamw_class);
+    case 11: return (int)sizeof(pdes_adamw_state);
     default: return -1;
   }
 }

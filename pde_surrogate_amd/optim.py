@@ -15,7 +15,8 @@ Two ways in, both without touching the loop body:
     plain `torch.optim.Adam` over exactly one such network's parameters, at its first step, into the subclass below
     (PDES_ADAM_AUTO_FUSED=1: only selects `fused=True` of the same class; =0 leaves it alone).
 
-Everything else of `torch.optim` is re-exported unchanged.
+`FusedAdamW` (AdamW over any list of parameters, states in 32 or 8 bits, clipping by the gradients' norm) and
+`clip_grad_norm_` come from adamw.py.  Everything else of `torch.optim` is re-exported unchanged.
 """
 import ctypes
 import math
@@ -26,6 +27,7 @@ from torch.optim import *                       # noqa: F401,F403  (the module s
 from torch.optim import Adam as _TorchAdam
 
 from . import _lib
+from .adamw import FusedAdamW, clip_grad_norm_   # noqa: F401
 
 
 def _owner(params):
