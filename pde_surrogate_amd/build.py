@@ -1,4 +1,5 @@
-"""Build libpdes_hip.so (all HIP kernels + the C ABI) in-tree with hipcc for gfx950.
+"""Build libpdes_hip.so (all HIP kernels + the C ABI) in-tree with hipcc for gfx950, and _tensor_list.so (host code that reads
+Python lists of tensors, against the installed torch's headers) with g++.
 
     python -m pde_surrogate_amd.build            # rebuild if any source is newer than the .so
     python -m pde_surrogate_amd.build --force
@@ -14,6 +15,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libpdes_hip.so')
+HOST_SRC = os.path.join(CSRC, 'tensor_list.cpp')
+HOST_LIB = os.path.join(HERE, '_tensor_list.so')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-ffp-contract=fast',
          '-Wno-unused-result', '-munsafe-fp-atomics']
 # added for one source: the list operators round every product and sum once (no contraction), and use no packed fp32
@@ -29,11 +32,25 @@ def headers():
     return glob.glob(os.path.join(CSRC, '*.h')) + glob.glob(os.path.join(CSRC, '*.inc')) + glob.glob(os.path.join(os.path.dirname(HERE), 'include', '*.h'))
 
 
+def needs_host_build():
+    return not os.path.exists(HOST_LIB) or os.path.getmtime(HOST_SRC) > os.path.getmtime(HOST_LIB)
+
+
 def needs_build():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or needs_host_build():
         return True
     t = os.path.getmtime(LIB)
     return any(os.path.getmtime(p) > t for p in sources() + headers())
+
+
+def host_command():
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    return ([os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
+             f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}'] + ['-I' + d for d in include_paths()] +
+            ['-I' + sysconfig.get_paths()['include'], HOST_SRC] + ['-L' + d for d in library_paths()] +
+            ['-ltorch_python', '-ltorch_cpu', '-lc10', '-o', HOST_LIB])
 
 
 def build(force=False, verbose=True):
@@ -41,6 +58,7 @@ def build(force=False, verbose=True):
         return LIB
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
     objs = []
+    host = subprocess.Popen(host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT) if force or needs_host_build() else None
     # one object per source, compiled in parallel, then linked: keeps rebuilds to seconds
     procs = []
     for src in sources():
@@ -57,6 +75,11 @@ def build(force=False, verbose=True):
         if p.returncode != 0:
             sys.stderr.write(out.decode())
             raise RuntimeError(f'hipcc failed on {src}')
+    if host is not None:
+        out, _ = host.communicate()
+        if host.returncode != 0:
+            sys.stderr.write(out.decode())
+            raise RuntimeError(f'{os.environ.get("CXX", "g++")} failed on {HOST_SRC}')
     cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC'] + objs + ['-o', LIB]
     if verbose:
         print(' '.join(cmd), flush=True)
