@@ -625,7 +625,7 @@ typedef struct pdes_adamw_state {
   short* low;             /* bf16 parameters: the 16 bits below each (nullable: parameters are rounded to nearest) */
   long long blocks;       /* blocks that the state buffers hold */
   const double* norm_rows;/* of pdes_grad_norm: gradients are multiplied by min(1, limit / (norm + 1e-6)) as they are read */
-  float* norm_out;        /* with norm_rows: the norm (nullable) */
+  float* norm_out;        /* with norm_rows: the norm is written here */
   void* hyper;            /* with step_dev: PDES_MT_HYPER_BYTES of device scratch */
   float limit;
   int dtype, bits, maximize;

@@ -1,7 +1,7 @@
 // Operators over many tensors in one launch: the AdamW step with 32-bit or 8-bit states, the common norm of a list of
 // gradients, and their clipping (include/pdes_hip.h: pdes_adamw_step, pdes_grad_norm, pdes_clip_grads).
 //
-// One workgroup walks over chunks of the concatenated list.  The list itself (addresses, lengths) travels BY VALUE in the
+// The list is cut into chunks, each inside one tensor; a workgroup of a step takes one.  The list itself (addresses, lengths) travels BY VALUE in the
 // kernel arguments, up to 96 tensors a launch: nothing to copy, no buffer that a later call could overwrite while an
 // earlier launch still reads it, and a captured graph holds its own copy.
 //
@@ -19,7 +19,7 @@ constexpr int MT_MAX = 96;                   // tensors of one launch
 constexpr int MT_CLASSES = PDES_MT_CLASSES;  // different sets of hyper-parameters of one launch
 constexpr int MT_ROWS = PDES_MT_ROWS;        // partial sums of the norm
 constexpr long long MT_LONGEST = 1ll << 40;  // elements of a list: chunks are counted in 32 bits
-constexpr int MT_TILE = 2048;                // elements that a workgroup of the step takes at a time: the unit of a chunk
+constexpr int MT_TILE = 2048;                // elements that a workgroup of the step takes at a time: eight a thread
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 // parameters and gradients are views anywhere in their buffers: their vector accesses need the element's alignment only
@@ -44,17 +44,18 @@ struct StepArgs {
   uint32_t chunk0[MT_MAX];      // first chunk of each tensor; unused entries hold 0xffffffff
   MtHyper h[MT_CLASSES];
   const MtHyper* hdev;          // captured steps: the same table in device memory
-  const double* partials;       // not NULL: clip by the norm that these rows add up to
-  float* norm_out;
+  const double* rows;           // clipping by the norm that these rows make (NULL: `norm` holds it already)
+  float* norm;                  // NULL: no clipping
   void* m;
   void* v;
   float* ms;
   float* rs;
   int16_t* low;
-  uint32_t chunks, tiles;       // chunks of this launch; tiles of a chunk
-  float limit, sign;
+  uint32_t chunks, tiles;       // chunks of this launch, a workgroup each; tiles of a chunk
+  float limit;
 };
 static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(MtHyper) * MT_CLASSES == PDES_MT_HYPER_BYTES, "pdes_adamw_state.hyper");
 
 constexpr int NORM_MAX = 160;
 struct NormArgs {
@@ -104,60 +105,75 @@ struct F16 {
   static __device__ __forceinline__ E down(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
 };
 
-// N consecutive elements of which `cnt` exist (the others read as zero and are not written)
-template <class T, int N>
+// Global accesses.  NT: streaming ones, for lists that are larger than the caches and will be gone from them before anybody asks
+// again (STEP_STREAMS, NORM_STREAMS).
+#define PDES_GLOBAL __attribute__((address_space(1)))
+template <bool NT, class W>
+__device__ __forceinline__ W get(const void* p, int k = 0) {
+  const PDES_GLOBAL W* q = (const PDES_GLOBAL W*)p + k;
+  if constexpr (NT) return __builtin_nontemporal_load(q);
+  return *q;
+}
+template <bool NT, class W>
+__device__ __forceinline__ void put(void* p, W w, int k = 0) {
+  PDES_GLOBAL W* q = (PDES_GLOBAL W*)p + k;
+  if constexpr (NT) __builtin_nontemporal_store(w, q);
+  else *q = w;
+}
+// N consecutive elements.  ALL: they exist; otherwise `cnt` of them do (the others read as zero and are not written).  The
+// whole-vector form is a plain global access without a branch, so that a thread's loads are all under way at once (fp32 norm
+// of 332 M elements: 368 us with a branch at each load, 222 us without)
+template <class T, int N, bool ALL, bool NT>
 __device__ __forceinline__ void load(const typename T::E* p, long long cnt, typename T::E (&x)[N]) {
-  if (cnt >= N) {
-    if constexpr (sizeof(typename T::E) == 4) {
+  typedef typename T::E E;
+  if constexpr (!ALL) {
+    if (cnt >= N) return load<T, N, true, NT>(p, cnt, x);
 #pragma unroll
-      for (int k = 0; k < N / 4; ++k) {
-        const f32x4_e w = reinterpret_cast<const f32x4_e*>(p)[k];
-        x[4 * k] = w[0]; x[4 * k + 1] = w[1]; x[4 * k + 2] = w[2]; x[4 * k + 3] = w[3];
-      }
-    } else if constexpr (N == 4) {
-      const u32x2_e w = *reinterpret_cast<const u32x2_e*>(p);
+    for (int k = 0; k < N; ++k) x[k] = k < cnt ? get<false, E>(p, k) : (E)0;
+  } else if constexpr (sizeof(E) == 4) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) { x[2 * k] = (uint16_t)w[k]; x[2 * k + 1] = (uint16_t)(w[k] >> 16); }
-    } else {
-#pragma unroll
-      for (int j = 0; j < N / 8; ++j) {
-        const u32x4_e w = reinterpret_cast<const u32x4_e*>(p)[j];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { x[8 * j + 2 * k] = (uint16_t)w[k]; x[8 * j + 2 * k + 1] = (uint16_t)(w[k] >> 16); }
-      }
+    for (int k = 0; k < N / 4; ++k) {
+      const f32x4_e w = get<NT, f32x4_e>(p, k);
+      x[4 * k] = w[0]; x[4 * k + 1] = w[1]; x[4 * k + 2] = w[2]; x[4 * k + 3] = w[3];
     }
-  } else {
+  } else if constexpr (N == 4) {
+    const u32x2_e w = get<NT, u32x2_e>(p);
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = k < cnt ? p[k] : (typename T::E)0;
+    for (int k = 0; k < 2; ++k) { x[2 * k] = (uint16_t)w[k]; x[2 * k + 1] = (uint16_t)(w[k] >> 16); }
+  } else {
+    static_assert(N == 8, "one 16-byte access");
+    const u32x4_e w = get<NT, u32x4_e>(p);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { x[2 * k] = (uint16_t)w[k]; x[2 * k + 1] = (uint16_t)(w[k] >> 16); }
   }
 }
-template <class T, int N>
+template <class T, int N, bool ALL, bool NT>
 __device__ __forceinline__ void store(typename T::E* p, long long cnt, const typename T::E (&x)[N]) {
-  if (cnt >= N) {
-    if constexpr (sizeof(typename T::E) == 4) {
-#pragma unroll
-      for (int k = 0; k < N / 4; ++k) {
-        const f32x4_e w = {x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
-        reinterpret_cast<f32x4_e*>(p)[k] = w;
-      }
-    } else if constexpr (N == 4) {
-      const u32x2_e w = {x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
-      *reinterpret_cast<u32x2_e*>(p) = w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < N / 8; ++j) {
-        u32x4_e w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = x[8 * j + 2 * k] | (uint32_t)x[8 * j + 2 * k + 1] << 16;
-        reinterpret_cast<u32x4_e*>(p)[j] = w;
-      }
-    }
-  } else {
+  typedef typename T::E E;
+  if constexpr (!ALL) {
+    if (cnt >= N) return store<T, N, true, NT>(p, cnt, x);
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (k < cnt) p[k] = x[k];
+      if (k < cnt) put<false, E>(p, x[k], k);
+  } else if constexpr (sizeof(E) == 4) {
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+      const f32x4_e w = {x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
+      put<NT>(p, w, k);
+    }
+  } else if constexpr (N == 4) {
+    const u32x2_e w = {x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
+    put<NT>(p, w);
+  } else {
+    static_assert(N == 8, "one 16-byte access");
+    u32x4_e w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = x[2 * k] | (uint32_t)x[2 * k + 1] << 16;
+    put<NT>(p, w);
   }
 }
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- the norm ----------------------------------------------------------------------------------------------------------
 // kind 2: sum of squares; kind 0: largest magnitude, NaN if any element is.  Sums are fp64 throughout (the squares of fp32
@@ -193,38 +209,64 @@ __device__ __forceinline__ float clip_factor(float norm, float limit) {
   return c > 1.f ? 1.f : c;
 }
 
-constexpr int NORM_THREADS = 512;
-template <class T, int KIND>
-__global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const NormArgs a) {
-  constexpr int V = 16 / sizeof(typename T::E);
-  constexpr int TILE = NORM_THREADS * V;       // one 16-byte access of every thread: a chunk is four of them
-  __shared__ double lds[NORM_THREADS / 64];
+template <class T, int KIND, int THREADS, int U, bool NT, bool ALL>
+__device__ __forceinline__ void norm_chunk(const typename T::E* g, long long left, double (&acc)[4]) {
+  constexpr int V = 16 / sizeof(typename T::E), TILE = THREADS * V;
+  typename T::E x[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) load<T, V, ALL, NT>(g + u * TILE, left - u * TILE, x[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const double d = (double)T::up(x[u][k]);
+      acc[k & 3] = KIND == 2 ? fma(d, d, acc[k & 3]) : join<0>(acc[k & 3], fabs(d));
+    }
+}
+// One workgroup a CU and row; a thread has U accesses of 16 bytes under way.  Bound by reading: 332 M elements of fp32 192 us =
+// 6.9 TB/s, of bf16 98 us = 6.8 TB/s (streaming), 214 and 113 us through the caches.
+template <class T, int KIND, int THREADS, int U, bool NT>
+__global__ __launch_bounds__(THREADS) void grad_norm_kernel(const NormArgs a) {
+  constexpr int V = 16 / sizeof(typename T::E), CHUNK = THREADS * V * U;
+  __shared__ double lds[THREADS / 64];
   const Finder<NORM_MAX> find(a.chunk0);
-  double acc = 0.0;
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};        // (four chains: one would wait for itself)
   for (uint32_t c = blockIdx.x; c < a.chunks; c += MT_ROWS) {
     const int at = __builtin_amdgcn_readfirstlane(find(c));
-    const typename T::E* g = static_cast<const typename T::E*>(a.g[at]);
-    const long long n = a.n[at], base = (long long)(c - a.chunk0[at]) * (4 * TILE) + (int)threadIdx.x * V;
-    typename T::E x[4][V];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load<T, V>(g + base + u * TILE, n - base - u * TILE, x[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const double d = (double)T::up(x[u][k]);
-        acc = KIND == 2 ? fma(d, d, acc) : join<0>(acc, fabs(d));
-      }
+    const long long base = (long long)(c - a.chunk0[at]) * CHUNK, left = a.n[at] - base;
+    const int mine = (int)threadIdx.x * V;
+    const typename T::E* g = static_cast<const typename T::E*>(a.g[at]) + base + mine;
+    if (left >= CHUNK) norm_chunk<T, KIND, THREADS, U, NT, true>(g, left - mine, acc);
+    else norm_chunk<T, KIND, THREADS, U, NT, false>(g, left - mine, acc);
   }
-  const double s = block_join<KIND, NORM_THREADS / 64>(acc, lds);
+  const double x = join<KIND>(join<KIND>(acc[0], acc[1]), join<KIND>(acc[2], acc[3]));
+  const double s = block_join<KIND, THREADS / 64>(x, lds);
   if (threadIdx.x == 0) a.out[blockIdx.x] = a.in ? join<KIND>(a.in[blockIdx.x], s) : s;
+}
+// the norm of the rows, for steps of many workgroups
+__global__ __launch_bounds__(MT_ROWS) void norm_kernel(const double* rows, float* norm) {
+  __shared__ double lds[4];
+  const float x = whole_norm<2>(rows, lds);
+  if (threadIdx.x == 0) *norm = x;
 }
 
 // gradients times the clipping factor; where that is 1 nothing is read or written
+template <class T, bool ALL>
+__device__ __forceinline__ void clip_chunk(typename T::E* g, long long left, float f) {
+  constexpr int V = 16 / sizeof(typename T::E), TILE = 256 * V;
+  typename T::E x[4][V];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) load<T, V, ALL, false>(g + u * TILE, left - u * TILE, x[u]);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[u][k] = T::down(T::up(x[u][k]) * f);
+    store<T, V, ALL, false>(g + u * TILE, left - u * TILE, x[u]);
+  }
+}
 template <class T, int KIND>
 __global__ __launch_bounds__(256) void clip_kernel(const NormArgs a) {
-  constexpr int V = 16 / sizeof(typename T::E);
-  constexpr int TILE = 256 * V;
+  constexpr int V = 16 / sizeof(typename T::E), CHUNK = 4 * 256 * V;
   __shared__ double lds[4];
   const float norm = whole_norm<KIND>(a.in, lds);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm_out) *a.norm_out = norm;
@@ -234,17 +276,11 @@ __global__ __launch_bounds__(256) void clip_kernel(const NormArgs a) {
   const Finder<NORM_MAX> find(a.chunk0);
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     const int at = __builtin_amdgcn_readfirstlane(find(c));
-    typename T::E* g = static_cast<typename T::E*>(a.g[at]);
-    const long long n = a.n[at], base = (long long)(c - a.chunk0[at]) * (4 * TILE) + (int)threadIdx.x * V;
-    typename T::E x[4][V];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load<T, V>(g + base + u * TILE, n - base - u * TILE, x[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[u][k] = T::down(T::up(x[u][k]) * f);
-      store<T, V>(g + base + u * TILE, n - base - u * TILE, x[u]);
-    }
+    const long long base = (long long)(c - a.chunk0[at]) * CHUNK, left = a.n[at] - base;
+    const int mine = (int)threadIdx.x * V;
+    typename T::E* g = static_cast<typename T::E*>(a.g[at]) + base + mine;
+    if (left >= CHUNK) clip_chunk<T, true>(g, left - mine, f);
+    else clip_chunk<T, false>(g, left - mine, f);
   }
 }
 
@@ -282,62 +318,93 @@ __device__ __forceinline__ float new_weight(float w, float m, float r, const MtH
   const float u = m / (r * h.rc2 + h.eps);
   return w * h.decay - u * h.step;
 }
-
-// factor of the gradients: -1 to maximise, times the clipping factor
-template <bool CLIP>
-__device__ __forceinline__ float grad_factor(const StepArgs& a, double* lds) {
-  if constexpr (!CLIP) return a.sign;
-  const float norm = whole_norm<2>(a.partials, lds);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm_out) *a.norm_out = norm;
-  return a.sign * clip_factor(norm, a.limit);
+// The same in the 8-bit kernel, which computes about as long as it waits for memory.  A weight that is rounded to 16 bits takes the
+// quotient from the reciprocal instruction (off by a place, 2^-23, where the weight's rounding is 2^-9 or 2^-12); the fix-up
+// gives the quotients of zeros, infinities and NaN.
+template <class T, bool LOW>
+__device__ __forceinline__ float new_weight(float w, float m, float r, const MtHyper& h) {
+  if constexpr (sizeof(typename T::E) == 4 || LOW) return new_weight(w, m, r, h);
+  const float den = r * h.rc2 + h.eps;
+  const float u = __builtin_amdgcn_div_fixupf(m * __builtin_amdgcn_rcpf(den), den, m);
+  return w * h.decay - u * h.step;
 }
 
-template <class T, bool LOW, bool CLIP>
+// what clipping multiplies the gradients by
+__device__ __forceinline__ float grad_factor(const StepArgs& a, double* lds) {
+  if (!a.norm) return 1.f;
+  if (!a.rows) return clip_factor(*(const PDES_GLOBAL float*)a.norm, a.limit);
+  const float norm = whole_norm<2>(a.rows, lds);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+  return clip_factor(norm, a.limit);
+}
+__device__ __forceinline__ MtHyper hyper_of(const StepArgs& a, int cls) {
+  if (!a.hdev) return a.h[cls];
+  MtHyper h;
+  const PDES_GLOBAL MtHyper* d = (const PDES_GLOBAL MtHyper*)a.hdev + cls;
+  h.decay = d->decay; h.step = d->step; h.rc2 = d->rc2; h.eps = d->eps;
+  h.b1 = d->b1; h.ob1 = d->ob1; h.b2 = d->b2; h.ob2 = d->ob2; h.key = d->key;
+  return h;
+}
+
+// a thread's share of a tile: twice four consecutive elements, 1024 elements apart.  All of its loads come first
+constexpr int V32 = MT_TILE / 1024;
+template <class T, bool LOW, bool NT, bool ALL>
+__device__ __forceinline__ void step32(typename T::E* p, const typename T::E* g, float* m, float* v, int16_t* low, int cnt, float gf,
+                                       const MtHyper& h) {
+  typename T::E pe[V32][4], ge[V32][4];
+  f32x4 mv[V32], vv[V32];
+  u32x2 lw[V32];
+#pragma unroll
+  for (int u = 0; u < V32; ++u) {
+    const int i = 1024 * u, left = cnt - i;
+    if (!ALL && left <= 0) continue;
+    load<T, 4, ALL, NT>(p + i, left, pe[u]);
+    load<T, 4, ALL, NT>(g + i, left, ge[u]);
+    mv[u] = get<NT, f32x4>(m + i);                         // (states are padded to a block)
+    vv[u] = get<NT, f32x4>(v + i);
+    if constexpr (LOW) lw[u] = get<NT, u32x2>(low + i);
+  }
+#pragma unroll
+  for (int u = 0; u < V32; ++u) {
+    const int i = 1024 * u, left = cnt - i;
+    if (!ALL && left <= 0) continue;
+    int16_t lo[4] = {};
+    if constexpr (LOW) { lo[0] = (int16_t)lw[u][0]; lo[1] = (int16_t)(lw[u][0] >> 16); lo[2] = (int16_t)lw[u][1]; lo[3] = (int16_t)(lw[u][1] >> 16); }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float gk = T::up(ge[u][k]) * gf;
+      mv[u][k] = mv[u][k] * h.b1 + gk * h.ob1;
+      vv[u][k] = vv[u][k] * h.b2 + gk * gk * h.ob2;
+      pe[u][k] = narrow<T, LOW>(new_weight(widen<T, LOW>(pe[u][k], lo[k]), mv[u][k], sqrtf(vv[u][k]), h), lo[k]);
+    }
+    store<T, 4, ALL, NT>(p + i, left, pe[u]);
+    put<NT>(m + i, mv[u]);
+    put<NT>(v + i, vv[u]);
+    if constexpr (LOW) {
+      const u32x2 w = {(uint16_t)lo[0] | (uint32_t)(uint16_t)lo[1] << 16, (uint16_t)lo[2] | (uint32_t)(uint16_t)lo[3] << 16};
+      put<NT>(low + i, w);
+    }
+  }
+}
+template <class T, bool LOW, bool NT>
 __global__ __launch_bounds__(256) void adamw32_kernel(const StepArgs a) {
   typedef typename T::E E;
   __shared__ double lds[4];
-  const float gf = grad_factor<CLIP>(a, lds);
+  const float gf = grad_factor(a, lds);
   const Finder<MT_MAX> find(a.chunk0);
-  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const int at = __builtin_amdgcn_readfirstlane(find(c));
-    const MtRef t = a.t[at];
-    const MtHyper h = a.hdev ? a.hdev[t.cls] : a.h[t.cls];
-    const long long n = (long long)((uint64_t)t.n_hi << 32 | t.n_lo), s0 = (long long)t.block0 * MT_BLOCK;
-    const long long base = (long long)(c - a.chunk0[at]) * a.tiles * MT_TILE;
-    E* const p = static_cast<E*>(t.p) + base;
-    const E* const g = static_cast<const E*>(t.g) + base;
-    float* const m = static_cast<float*>(a.m) + s0 + base;
-    float* const v = static_cast<float*>(a.v) + s0 + base;
-    int16_t* const low = LOW ? a.low + s0 + base : nullptr;
-    const long long left = n - base;
-    const int end = (int)(left < (long long)a.tiles * MT_TILE ? left : (long long)a.tiles * MT_TILE);
-    for (int i = threadIdx.x * 4; i < end; i += 1024) {
-      E pe[4], ge[4];
-      int16_t lw[4] = {};
-      load<T, 4>(p + i, end - i, pe);
-      load<T, 4>(g + i, end - i, ge);
-      f32x4 mv = *reinterpret_cast<const f32x4*>(m + i), vv = *reinterpret_cast<const f32x4*>(v + i);   // (states are padded to a block)
-      if constexpr (LOW) {
-        const uint2 w = *reinterpret_cast<const uint2*>(low + i);
-        lw[0] = (int16_t)w.x; lw[1] = (int16_t)(w.x >> 16); lw[2] = (int16_t)w.y; lw[3] = (int16_t)(w.y >> 16);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float gk = T::up(ge[k]) * gf;
-        mv[k] = mv[k] * h.b1 + gk * h.ob1;
-        vv[k] = vv[k] * h.b2 + gk * gk * h.ob2;
-        const float w = new_weight(widen<T, LOW>(pe[k], lw[k]), mv[k], sqrtf(vv[k]), h);
-        pe[k] = narrow<T, LOW>(w, lw[k]);
-      }
-      store<T, 4>(p + i, end - i, pe);
-      *reinterpret_cast<f32x4*>(m + i) = mv;
-      *reinterpret_cast<f32x4*>(v + i) = vv;
-      if constexpr (LOW) {
-        const uint2 w = make_uint2((uint16_t)lw[0] | (uint32_t)(uint16_t)lw[1] << 16, (uint16_t)lw[2] | (uint32_t)(uint16_t)lw[3] << 16);
-        *reinterpret_cast<uint2*>(low + i) = w;
-      }
-    }
-  }
+  const int at = __builtin_amdgcn_readfirstlane(find(blockIdx.x));
+  const MtRef t = a.t[at];
+  const MtHyper h = hyper_of(a, t.cls);
+  const long long n = (long long)((uint64_t)t.n_hi << 32 | t.n_lo), base = (long long)(blockIdx.x - a.chunk0[at]) * MT_TILE, left = n - base;
+  const long long s = (long long)t.block0 * MT_BLOCK + base;
+  const uint32_t mine = threadIdx.x * 4;
+  E* const p = static_cast<E*>(t.p) + base + mine;
+  const E* const g = static_cast<const E*>(t.g) + base + mine;
+  float* const m = static_cast<float*>(a.m) + s + mine;
+  float* const v = static_cast<float*>(a.v) + s + mine;
+  int16_t* const low = LOW ? a.low + s + mine : nullptr;
+  if (left >= MT_TILE) step32<T, LOW, NT, true>(p, g, m, v, low, MT_TILE, gf, h);
+  else step32<T, LOW, NT, false>(p, g, m, v, low, (int)left - (int)mine, gf, h);
 }
 
 // 8-bit states.  Blocks of 256 elements of one tensor share an fp32 scale = (largest value) / 448, and m and r = sqrt(v) are
@@ -356,124 +423,212 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   x ^= x >> 16;
   return x;
 }
-// the largest magnitude among the 32 lanes of a half wave, as fp32 bits
-__device__ __forceinline__ uint32_t half_max(uint32_t x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
-    x = x > y ? x : y;
-  }
+// The largest magnitudes of a half wave's block: a lane brings those of its m and r, as bits; lanes 0 .. 15 get the block's
+// for m, lanes 16 .. 31 its for r.  One exchange of the rows sorts m into the first and r into the second, then both are
+// reduced in their row at once (DPP); the scale and its inverse are found once in each row instead of twice in every lane.
+__device__ __forceinline__ uint32_t row_tops(uint32_t m, uint32_t r) {
+  const auto rows = __builtin_amdgcn_permlane16_swap(m, r, false, false);
+  uint32_t x = rows[0] > rows[1] ? rows[0] : rows[1];
+#define PDES_MAX_DPP(ctrl) { const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xf, 0xf, true); x = x > y ? x : y; }
+  PDES_MAX_DPP(0xB1)       // lanes 1 0 3 2
+  PDES_MAX_DPP(0x4E)       // lanes 2 3 0 1
+  PDES_MAX_DPP(0x141)      // eight lanes mirrored
+  PDES_MAX_DPP(0x140)      // sixteen lanes mirrored
+#undef PDES_MAX_DPP
   return x;
 }
-// scale of a block and what its values are multiplied by, from its largest value
-__device__ __forceinline__ void scales(uint32_t top_bits, float& scale, float& inverse) {
-  const float top = __uint_as_float(top_bits);
-  const bool live = top >= 0x1p-100f;          // under that the scale's own arithmetic would be subnormal: held as zeros
-  scale = live ? top * (1.f / 448.f) : 0.f;
-  inverse = live ? 448.f / top : 0.f;
+// 448 / top, correctly rounded: the reciprocal, one step of Newton's for it and two corrections of the quotient.  (The division
+// operator scales its operands besides; here they and all that is between are normal numbers: 2^-100 <= top <= 2^120.)
+__device__ __forceinline__ float inverse_scale(float top) {
+  float y = __builtin_amdgcn_rcpf(top);
+  y = fmaf(fmaf(-top, y, 1.f), y, y);
+  float q = 448.f * y;
+  q = fmaf(fmaf(-q, top, 448.f), y, q);
+  return fmaf(fmaf(-q, top, 448.f), y, q);
 }
-// e4m3 code of |x| * inverse, rounded down after `noise` / 2^20 of a spacing was added.  The product with 2^-120 puts e4m3's
-// exponents (bias 7) where fp32's lie (bias 127), its subnormal range included: the code is the upper bits.
-__device__ __forceinline__ uint32_t to_code(uint32_t mag_bits, float inverse, uint32_t noise) {
-  const float y = __uint_as_float(mag_bits) * inverse * 0x1p-120f;
-  const uint32_t code = (__float_as_uint(y) + noise) >> 20;
-  return code < 0x7Eu ? code : 0x7Eu;
-}
+constexpr uint32_t TOP_LEAST = 0x0d800000u, TOP_MOST = 0x7b800000u;      // 2^-100 and 2^120 as bits
 __device__ __forceinline__ void unpack8(uint32_t w, float scale, float* x) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
   x[0] = a[0] * scale; x[1] = a[1] * scale; x[2] = b[0] * scale; x[3] = b[1] * scale;
 }
+// sqrtf, correctly rounded for x >= 2^-96: the hardware's root is off by one place at most, and the signs of x - s s' for its
+// two neighbours s' say which of the three is nearest.  (What sqrtf does besides is scaling for small x.  There the result is
+// off by a place at most, and subnormal x go through sqrtf itself.)  0, infinity and NaN come out as they are: the neighbours'
+// residuals are NaN or zero and change nothing.
+__device__ __forceinline__ float root(float x) {
+  const float s = __builtin_amdgcn_sqrtf(x);
+  const float under = __uint_as_float(__float_as_uint(s) - 1u), over = __uint_as_float(__float_as_uint(s) + 1u);
+  float r = fmaf(-under, s, x) <= 0.f ? under : s;
+  return fmaf(-over, s, x) > 0.f ? over : r;
+}
+constexpr int SUBNORMAL = 0x90;              // class mask: subnormal numbers of either sign
 
-template <class T, bool LOW, bool CLIP>
-__global__ __launch_bounds__(256) void adamw8_kernel(const StepArgs a) {
+// A half wave holds a block, a lane eight elements of it: consecutive ones of 16 bits, or twice four of 32 bits, 128 elements
+// apart, so that each access of a wave covers whole lines (332 M fp32 parameters, streaming: 852 us; eight consecutive ones, two
+// accesses to each half of a line: 975 us). 
+template <class T>
+struct Share {
+  static constexpr int PER = sizeof(typename T::E) == 4 ? 4 : 8, PARTS = 8 / PER, APART = 128;
+  // the place of a lane's element k in its block
+  static __device__ __forceinline__ uint32_t place(int lane, int k) { return lane * PER + k % PER + k / PER * APART; }
+};
+template <class T, bool ALL, bool NT>
+__device__ __forceinline__ void load8(const typename T::E* p, long long cnt, typename T::E (&x)[8]) {
+  constexpr int PER = Share<T>::PER;
+#pragma unroll
+  for (int j = 0; j < Share<T>::PARTS; ++j) {
+    typename T::E part[PER];
+    load<T, PER, ALL, NT>(p + j * Share<T>::APART, cnt - j * Share<T>::APART, part);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[j * PER + k] = part[k];
+  }
+}
+template <class T, bool ALL, bool NT>
+__device__ __forceinline__ void store8(typename T::E* p, long long cnt, const typename T::E (&x)[8]) {
+  constexpr int PER = Share<T>::PER;
+#pragma unroll
+  for (int j = 0; j < Share<T>::PARTS; ++j) {
+    typename T::E part[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) part[k] = x[j * PER + k];
+    store<T, PER, ALL, NT>(p + j * Share<T>::APART, cnt - j * Share<T>::APART, part);
+  }
+}
+template <class T, bool NT>
+__device__ __forceinline__ u32x2 get_codes(const uint8_t* q) {
+  if constexpr (Share<T>::PARTS == 1) return get<NT, u32x2>(q);
+  const u32x2 w = {get<NT, uint32_t>(q), get<NT, uint32_t>(q + Share<T>::APART)};
+  return w;
+}
+template <class T, bool NT>
+__device__ __forceinline__ void put_codes(uint8_t* q, u32x2 w) {
+  if constexpr (Share<T>::PARTS == 1) {
+    put<NT>(q, w);
+  } else {
+    put<NT, uint32_t>(q, w[0]);
+    put<NT, uint32_t>(q + Share<T>::APART, w[1]);
+  }
+}
+
+template <class T, bool LOW, bool CLIP, bool NT, bool ALL>
+__device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, uint8_t* mq, uint8_t* rq, float* ms, float* rs, int16_t* low,
+                                      long long cnt, float gf, const MtHyper& h, uint32_t key, int lane) {
+  typename T::E pe[8], ge[8];
+  int16_t lw[8] = {};
+  load8<T, ALL, NT>(p, cnt, pe);
+  load8<T, ALL, NT>(g, cnt, ge);
+  const u32x2 mw = get_codes<T, NT>(mq), rw = get_codes<T, NT>(rq);
+  const float m_scale = get<false, float>(ms), r_scale = get<false, float>(rs);
+  if constexpr (LOW) {
+    const u32x4 w = get<NT, u32x4>(low);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { lw[2 * k] = (int16_t)w[k]; lw[2 * k + 1] = (int16_t)(w[k] >> 16); }
+  }
+  float m[8], r[8], v[8];
+  unpack8(mw[0], m_scale, m); unpack8(mw[1], m_scale, m + 4);
+  unpack8(rw[0], r_scale, r); unpack8(rw[1], r_scale, r + 4);
+  bool small = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float gk = CLIP ? T::up(ge[k]) * gf : T::up(ge[k]);
+    m[k] = m[k] * h.b1 + gk * h.ob1;
+    v[k] = r[k] * r[k] * h.b2 + gk * gk * h.ob2;
+    r[k] = root(v[k]);
+    small |= __builtin_amdgcn_classf(v[k], SUBNORMAL);
+  }
+  if (small) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r[k] = sqrtf(v[k]);
+  }
+  uint32_t mtop = 0, rtop = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    pe[k] = narrow<T, LOW>(new_weight<T, LOW>(widen<T, LOW>(pe[k], lw[k]), m[k], r[k], h), lw[k]);
+    const uint32_t mb = __float_as_uint(m[k]) & 0x7fffffffu, rb = __float_as_uint(r[k]);
+    mtop = mb > mtop ? mb : mtop;
+    rtop = rb > rtop ? rb : rtop;              // (r is not negative; a NaN with the sign is the largest as well)
+  }
+  store8<T, ALL, NT>(p, cnt, pe);
+  if constexpr (LOW) {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint16_t)lw[2 * k] | (uint32_t)(uint16_t)lw[2 * k + 1] << 16;
+    put<NT>(low, w);
+  }
+  uint32_t top = row_tops(mtop, rtop);
+  const bool odd = __any(top > TOP_MOST);      // values that are not finite, or too large for inverse_scale
+  float scale, inverse;
+  if (!odd) {
+    const bool live = top >= TOP_LEAST;        // under that the scale's own arithmetic would be subnormal: held as zeros
+    scale = live ? __uint_as_float(top) * (1.f / 448.f) : 0.f;
+    inverse = live ? inverse_scale(__uint_as_float(top)) : 0.f;
+  } else {
+    mtop = rtop = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t mb = __float_as_uint(m[k]) & 0x7fffffffu, rb = __float_as_uint(r[k]) & 0x7fffffffu;
+      if (mb < 0x7f800000u && mb > mtop) mtop = mb;
+      if (rb < 0x7f800000u && rb > rtop) rtop = rb;
+    }
+    top = row_tops(mtop, rtop);
+    scale = top >= TOP_LEAST ? __uint_as_float(top) * (1.f / 448.f) : 0.f;
+    inverse = top >= TOP_LEAST ? 448.f / __uint_as_float(top) : 0.f;
+  }
+  if ((lane & 15) == 0) put<false>(lane ? rs : ms, scale);
+  const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(inverse), __float_as_uint(inverse), false, false);
+  const float mi = __uint_as_float(both[0]), ri = __uint_as_float(both[1]);
+  u32x2 mo = {0, 0}, ro = {0, 0};
+  // the conversion drops 20 bits of the number (more under 2^-6) after the upper 20 bits of `z` have been added to them: rounding
+  // down after z / 2^32 of a spacing was added, up to the bits behind 2^-29 of a number under 2^-6, which it cuts
+#define PDES_HOLD(k, word, byte)                                                                                        \
+  {                                                                                                                     \
+    const uint32_t z = mix(key + GOLD * Share<T>::place(lane, k));                                                                 \
+    mo[word] = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(__builtin_amdgcn_fmed3f(m[k] * mi, -448.f, 448.f), (int)z, (int)mo[word], byte); \
+    ro[word] = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(__builtin_amdgcn_fmed3f(r[k] * ri, r[k] > 0.f ? 0x1p-9f : 0.f, 448.f), (int)(z << 12), (int)ro[word], byte); \
+  }
+  PDES_HOLD(0, 0, 0) PDES_HOLD(1, 0, 1) PDES_HOLD(2, 0, 2) PDES_HOLD(3, 0, 3)
+  PDES_HOLD(4, 1, 0) PDES_HOLD(5, 1, 1) PDES_HOLD(6, 1, 2) PDES_HOLD(7, 1, 3)
+#undef PDES_HOLD
+  if (odd) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t nan = 0x7fu << (8 * (k & 3)), sign = 0x80u << (8 * (k & 3));
+      if ((__float_as_uint(m[k]) & 0x7fffffffu) >= 0x7f800000u)
+        mo[k >> 2] = (mo[k >> 2] & ~sign) | nan | ((__float_as_uint(m[k]) >> 31) ? sign : 0u);
+      if ((__float_as_uint(r[k]) & 0x7fffffffu) >= 0x7f800000u) ro[k >> 2] = (ro[k >> 2] & ~sign) | nan;
+    }
+  }
+  put_codes<T, NT>(mq, mo);
+  put_codes<T, NT>(rq, ro);
+}
+
+template <class T, bool LOW, bool CLIP, bool NT>
+__global__ __launch_bounds__(256, sizeof(typename T::E) == 2 && !LOW ? 5 : 1) void adamw8_kernel(const StepArgs a) {
   typedef typename T::E E;
   __shared__ double lds[4];
-  const float gf = grad_factor<CLIP>(a, lds);
+  const float gf = CLIP ? grad_factor(a, lds) : 1.f;
   const Finder<MT_MAX> find(a.chunk0);
-  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5;       // a half wave takes a block, a lane eight elements of it
-  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const int at = __builtin_amdgcn_readfirstlane(find(c));
-    const MtRef t = a.t[at];
-    const MtHyper h = a.hdev ? a.hdev[t.cls] : a.h[t.cls];
-    const long long n = (long long)((uint64_t)t.n_hi << 32 | t.n_lo);
-    const uint32_t blocks = (uint32_t)((n + MT_BLOCK - 1) / MT_BLOCK), first = (c - a.chunk0[at]) * a.tiles * (MT_TILE / MT_BLOCK);
-    const uint32_t many = a.tiles * (MT_TILE / MT_BLOCK), stop = blocks - first < many ? blocks : first + many;
-    const uint32_t tensor_key = mix(h.key + GOLD * (t.ordinal + 1));
-    for (uint32_t b = first + half; b < stop; b += 8) {
-      const long long i = (long long)b * MT_BLOCK + lane * 8, cnt = n - i;
-      const long long sb = (long long)t.block0 + b, s = sb * MT_BLOCK + lane * 8;
-      E* const p = static_cast<E*>(t.p) + i;
-      E pe[8], ge[8];
-      int16_t lw[8] = {};
-      load<T, 8>(p, cnt, pe);
-      load<T, 8>(static_cast<const E*>(t.g) + i, cnt, ge);
-      const uint2 mq = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s);
-      const uint2 rq = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s);
-      const float ms = a.ms[sb], rs = a.rs[sb];
-      if constexpr (LOW) {
-        const uint4 w = *reinterpret_cast<const uint4*>(a.low + s);
-        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { lw[2 * k] = (int16_t)q[k]; lw[2 * k + 1] = (int16_t)(q[k] >> 16); }
-      }
-      float m[8], r[8];
-      unpack8(mq.x, ms, m); unpack8(mq.y, ms, m + 4);
-      unpack8(rq.x, rs, r); unpack8(rq.y, rs, r + 4);
-      uint32_t mb[8], rb[8], mtop = 0, rtop = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float gk = T::up(ge[k]) * gf;
-        m[k] = m[k] * h.b1 + gk * h.ob1;
-        r[k] = sqrtf(r[k] * r[k] * h.b2 + gk * gk * h.ob2);
-        pe[k] = narrow<T, LOW>(new_weight(widen<T, LOW>(pe[k], lw[k]), m[k], r[k], h), lw[k]);
-        mb[k] = __float_as_uint(m[k]) & 0x7fffffffu;
-        rb[k] = __float_as_uint(r[k]) & 0x7fffffffu;
-        mtop = mb[k] > mtop ? mb[k] : mtop;
-        rtop = rb[k] > rtop ? rb[k] : rtop;
-      }
-      store<T, 8>(p, cnt, pe);
-      if constexpr (LOW) {
-        uint32_t q[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = (uint16_t)lw[2 * k] | (uint32_t)(uint16_t)lw[2 * k + 1] << 16;
-        *reinterpret_cast<uint4*>(a.low + s) = make_uint4(q[0], q[1], q[2], q[3]);
-      }
-      mtop = half_max(mtop);
-      rtop = half_max(rtop);
-      const bool bad = mtop >= 0x7f800000u || rtop >= 0x7f800000u;         // the same in all lanes of the half wave
-      if (bad) {
-        mtop = rtop = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (mb[k] < 0x7f800000u && mb[k] > mtop) mtop = mb[k];
-          if (rb[k] < 0x7f800000u && rb[k] > rtop) rtop = rb[k];
-        }
-        mtop = half_max(mtop);
-        rtop = half_max(rtop);
-      }
-      float nms, mi, nrs, ri;
-      scales(mtop, nms, mi);
-      scales(rtop, nrs, ri);
-      const uint32_t key = mix(tensor_key + GOLD * b);
-      uint32_t mc[8], rc[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t z = mix(key + GOLD * (uint32_t)(lane * 8 + k));
-        mc[k] = to_code(mb[k], mi, z >> 12);
-        rc[k] = to_code(rb[k], ri, z & 0xfffffu);
-        rc[k] = rc[k] ? rc[k] : rb[k] ? 1u : 0u;
-        if (bad) {
-          if (mb[k] >= 0x7f800000u) mc[k] = 0x7fu;
-          if (rb[k] >= 0x7f800000u) rc[k] = 0x7fu;
-        }
-        mc[k] |= (__float_as_uint(m[k]) >> 24) & 0x80u;
-      }
-      const uint2 mo = make_uint2(mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24, mc[4] | mc[5] << 8 | mc[6] << 16 | mc[7] << 24);
-      const uint2 ro = make_uint2(rc[0] | rc[1] << 8 | rc[2] << 16 | rc[3] << 24, rc[4] | rc[5] << 8 | rc[6] << 16 | rc[7] << 24);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = mo;
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = ro;
-      if (lane == 0) { a.ms[sb] = nms; a.rs[sb] = nrs; }
-    }
+  const int lane = threadIdx.x & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = threadIdx.x >> 5;
+  const uint32_t mine = half * MT_BLOCK + lane * Share<T>::PER;
+  const int at = __builtin_amdgcn_readfirstlane(find(blockIdx.x));
+  const MtRef t = a.t[at];
+  const MtHyper h = hyper_of(a, t.cls);
+  const long long n = (long long)((uint64_t)t.n_hi << 32 | t.n_lo);
+  const uint32_t tensor_key = mix(h.key + GOLD * (t.ordinal + 1)), tile0 = (blockIdx.x - a.chunk0[at]) * a.tiles;
+  for (uint32_t tile = tile0; tile < tile0 + a.tiles; ++tile) {
+    const long long i = (long long)tile * MT_TILE, left = n - i;
+    if (left <= 0) break;
+    const uint32_t b = tile * (MT_TILE / MT_BLOCK) + 2 * wave;               // of the wave's lower half
+    const uint32_t key0 = mix(tensor_key + GOLD * b), key1 = mix(tensor_key + GOLD * (b + 1)), key = half & 1 ? key1 : key0;
+    const long long s = (long long)t.block0 * MT_BLOCK + i, sb = t.block0 + (long long)tile * (MT_TILE / MT_BLOCK) + half;
+    E* const p = static_cast<E*>(t.p) + i + mine;
+    const E* const g = static_cast<const E*>(t.g) + i + mine;
+    uint8_t* const mq = static_cast<uint8_t*>(a.m) + s + mine;
+    uint8_t* const rq = static_cast<uint8_t*>(a.v) + s + mine;
+    int16_t* const low = LOW ? a.low + s + mine : nullptr;
+    if (left >= MT_TILE) step8<T, LOW, CLIP, NT, true>(p, g, mq, rq, a.ms + sb, a.rs + sb, low, 8, gf, h, key, lane);
+    else if (half * MT_BLOCK < (int)left)
+      step8<T, LOW, CLIP, NT, false>(p, g, mq, rq, a.ms + sb, a.rs + sb, low, (int)left - (int)mine, gf, h, key, lane);
   }
 }
 
@@ -484,15 +639,16 @@ struct ClassArgs {
   float* step_dev[MT_CLASSES];
   MtHyper* out;
   uint32_t seed;
-  int n;
+  int n, maximize;
 };
-__host__ __device__ __forceinline__ MtHyper constants(double lr, double b1, double b2, double eps, double wd, long long t, uint32_t seed) {
+__host__ __device__ __forceinline__ MtHyper constants(double lr, double b1, double b2, double eps, double wd, bool maximize, long long t, uint32_t seed) {
   MtHyper h;
   h.decay = (float)(1.0 - lr * wd);
   h.step = (float)(lr / (1.0 - pow(b1, (double)t)));
   h.rc2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
   h.eps = (float)eps;
-  h.b1 = (float)b1; h.ob1 = (float)(1.0 - b1);
+  h.b1 = (float)b1;
+  h.ob1 = (float)(maximize ? b1 - 1.0 : 1.0 - b1);           // (of the gradient, only its sign in m differs)
   h.b2 = (float)b2; h.ob2 = (float)(1.0 - b2);
   h.key = mix(seed + GOLD * (uint32_t)t);
   return h;
@@ -502,9 +658,18 @@ __global__ __launch_bounds__(64) void adamw_count_kernel(const ClassArgs a) {
   if (k >= a.n) return;
   const float t = *a.step_dev[k] + 1.f;
   *a.step_dev[k] = t;
-  a.out[k] = constants(a.lr_dev[k] ? (double)*a.lr_dev[k] : a.lr[k], a.b1[k], a.b2[k], a.eps[k], a.wd[k], (long long)t, a.seed);
+  a.out[k] = constants(a.lr_dev[k] ? (double)*a.lr_dev[k] : a.lr[k], a.b1[k], a.b2[k], a.eps[k], a.wd[k], a.maximize, (long long)t, a.seed);
 }
 
+constexpr long long LONG_LIST = 8ll << 20;
+// Tiles of a workgroup.  One, so that the workgroups walk through memory side by side (332 M fp32 elements: 1,749 us, with four
+// 1,790; 8-bit states: 919 and 1,011) -- but 16-bit elements with 8-bit states, which take as long to compute as to load, save
+// the look-up and the table's loads by two from 8 M and four from 64 M elements on (bf16, 128 M: 238 / 231 / 228 us with 1 / 2 / 4;
+// 32 M: 59.9 / 59.4 / 61.9; 4 M: 11.3 / 12.0 / 13.1)
+static uint32_t tiles_of(int bits, int size, long long total) {
+  if (bits == 32 || size == 4 || total < LONG_LIST) return 1;
+  return total < 8 * LONG_LIST ? 2 : 4;
+}
 static int item_size(int dtype) { return dtype == PDES_MT_F32 ? 4 : 2; }
 
 // one launch over grads[at .. at + count): fills the table, returns the number of tensors that went into it or an error
@@ -529,12 +694,25 @@ static int fill(NormArgs& a, const unsigned long long* grads, const long long* s
   return PDES_OK;
 }
 
-template <class T>
-static void launch_norm(int kind, const NormArgs& a, hipStream_t st) {
-  if (kind == 2)
-    hipLaunchKernelGGL((grad_norm_kernel<T, 2>), dim3(MT_ROWS), dim3(NORM_THREADS), 0, st, a);
+// Lists up to 4 MiB, a pass of the chip: 256 threads and chunks of 16 KiB (0.7 M fp32 elements 3.8 us; 5.8 us with the others'
+// shape).  Longer ones: 1024 threads and 64 KiB.  Streaming from 512 MiB on, twice the last-level cache: under it the optimiser's
+// step that follows finds part of the gradients there (norm and step of 100 M fp32 elements: 525 us, streaming 535; from 300 M
+// elements on streaming is the faster by a per cent, and by a tenth for the norm alone).
+constexpr int LONG_THREADS = 1024, SHORT_THREADS = 256, NORM_U = 4;
+constexpr long long SHORT_MOST = 16ll * MT_ROWS * SHORT_THREADS * NORM_U, NORM_STREAMS = 512ll << 20;
+template <class T, int KIND>
+static void launch_norm_kind(long long bytes, const NormArgs& a, hipStream_t st) {
+  if (bytes > NORM_STREAMS)
+    hipLaunchKernelGGL((grad_norm_kernel<T, KIND, LONG_THREADS, NORM_U, true>), dim3(MT_ROWS), dim3(LONG_THREADS), 0, st, a);
+  else if (bytes > SHORT_MOST)
+    hipLaunchKernelGGL((grad_norm_kernel<T, KIND, LONG_THREADS, NORM_U, false>), dim3(MT_ROWS), dim3(LONG_THREADS), 0, st, a);
   else
-    hipLaunchKernelGGL((grad_norm_kernel<T, 0>), dim3(MT_ROWS), dim3(NORM_THREADS), 0, st, a);
+    hipLaunchKernelGGL((grad_norm_kernel<T, KIND, SHORT_THREADS, NORM_U, false>), dim3(MT_ROWS), dim3(SHORT_THREADS), 0, st, a);
+}
+template <class T>
+static void launch_norm(int kind, long long bytes, const NormArgs& a, hipStream_t st) {
+  if (kind == 2) launch_norm_kind<T, 2>(bytes, a, st);
+  else launch_norm_kind<T, 0>(bytes, a, st);
 }
 template <class T>
 static void launch_clip(int kind, const NormArgs& a, hipStream_t st) {
@@ -545,19 +723,27 @@ static void launch_clip(int kind, const NormArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((clip_kernel<T, 0>), dim3(grid), dim3(256), 0, st, a);
 }
 
+// Streaming accesses for steps that touch more than this: with less, parts are still in the 256 MiB cache at the next step
+// (8 M fp32 elements = 122 MiB: 41 us streaming, 46 not; 4 M: 22 and 18).
+constexpr long long STEP_STREAMS = 96ll << 20;
+// Streaming steps with 32-bit states run best with two (fp32) or three (16-bit) workgroups on a CU, 64 to 84 KiB of loads under
+// way: the memory keeps fewer pages open (332 M fp32 elements: 1,529 us with two, 1,571 with three, 1,603 with four, 1,645
+// with the seven that the registers allow; bf16: 1,184 us with three, 1,270 with seven, 1,335 with two).  Unused LDS holds the others off.
+constexpr unsigned HOLD_TWO = 80000, HOLD_THREE = 53000;
+template <class T, bool LOW, bool NT>
+static void launch_step(int bits, const StepArgs& a, hipStream_t st) {
+  const unsigned hold = !NT ? 0 : sizeof(typename T::E) == 4 ? HOLD_TWO : HOLD_THREE;
+  if (bits == 32)
+    hipLaunchKernelGGL((adamw32_kernel<T, LOW, NT>), dim3(a.chunks), dim3(256), hold, st, a);
+  else if (a.norm)
+    hipLaunchKernelGGL((adamw8_kernel<T, LOW, true, NT>), dim3(a.chunks), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((adamw8_kernel<T, LOW, false, NT>), dim3(a.chunks), dim3(256), 0, st, a);
+}
 template <class T, bool LOW>
-static void launch_step(int bits, const StepArgs& a, unsigned grid, hipStream_t st) {
-  if (bits == 32) {
-    if (a.partials)
-      hipLaunchKernelGGL((adamw32_kernel<T, LOW, true>), dim3(grid), dim3(256), 0, st, a);
-    else
-      hipLaunchKernelGGL((adamw32_kernel<T, LOW, false>), dim3(grid), dim3(256), 0, st, a);
-  } else {
-    if (a.partials)
-      hipLaunchKernelGGL((adamw8_kernel<T, LOW, true>), dim3(grid), dim3(256), 0, st, a);
-    else
-      hipLaunchKernelGGL((adamw8_kernel<T, LOW, false>), dim3(grid), dim3(256), 0, st, a);
-  }
+static void launch_step(int bits, long long bytes, const StepArgs& a, hipStream_t st) {
+  if (bytes > STEP_STREAMS) launch_step<T, LOW, true>(bits, a, st);
+  else launch_step<T, LOW, false>(bits, a, st);
 }
 
 }  // namespace pdes
@@ -570,16 +756,20 @@ extern "C" int pdes_grad_norm(const unsigned long long* grads, const long long* 
   hipStream_t st = static_cast<hipStream_t>(stream);
   NormArgs a;
   a.out = rows; a.norm_out = nullptr; a.limit = 0.f;
+  long long total = 0;
+  for (int k = 0; k < count; ++k) total += sizes[k] > 0 && sizes[k] < MT_LONGEST ? sizes[k] : 0;
+  const long long bytes = total * item_size(dtype), 
+                  chunk = (bytes > SHORT_MOST ? LONG_THREADS : SHORT_THREADS) * NORM_U * 16ll / item_size(dtype);
   int done = 0;
   do {                            // (an empty list still writes its rows)
     int taken;
-    const int rc = fill(a, grads + done, sizes + done, count - done, dtype, 4ll * NORM_THREADS * (16 / item_size(dtype)), taken);
+    const int rc = fill(a, grads + done, sizes + done, count - done, dtype, chunk, taken);
     if (rc) return rc;
     a.in = add || done ? rows : nullptr;
     done += taken;
-    if (dtype == PDES_MT_F32) launch_norm<F32>(kind, a, st);
-    else if (dtype == PDES_MT_BF16) launch_norm<BF16>(kind, a, st);
-    else launch_norm<F16>(kind, a, st);
+    if (dtype == PDES_MT_F32) launch_norm<F32>(kind, bytes, a, st);
+    else if (dtype == PDES_MT_BF16) launch_norm<BF16>(kind, bytes, a, st);
+    else launch_norm<F16>(kind, bytes, a, st);
     PDES_LAUNCH_CHECK();
   } while (done < count);
   return PDES_OK;
@@ -613,7 +803,7 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
   if (count < 0 || !state || nclasses <= 0 || nclasses > MT_CLASSES || !classes || (count && (!params || !grads || !tensors))) return PDES_EINVAL;
   const pdes_adamw_state& s = *state;
   if (s.dtype < 0 || s.dtype > 2 || (s.bits != 32 && s.bits != 8) || (s.low && s.dtype != PDES_MT_BF16)) return PDES_EINVAL;
-  if (s.blocks < 0 || s.blocks > 0xffffffffll || (s.norm_rows && !(s.limit >= 0.f))) return PDES_EINVAL;
+  if (s.blocks < 0 || s.blocks > 0xffffffffll || (s.norm_rows && (!s.norm_out || !(s.limit >= 0.f)))) return PDES_EINVAL;
   if (s.blocks && (!s.exp_avg || !s.exp_avg_sq || (s.bits == 8 && (!s.exp_avg_scale || !s.rms_scale)))) return PDES_EINVAL;
   if (!aligned16(s.exp_avg) || !aligned16(s.exp_avg_sq) || !aligned16(s.low)) return PDES_EALIGN;
   const bool captured = classes[0].step_dev != nullptr;
@@ -624,7 +814,7 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     if ((c.step_dev != nullptr) != captured || (!captured && (c.step < 1 || c.lr_dev))) return PDES_EINVAL;
   }
   const int size = item_size(s.dtype);
-  long long total = 0;
+  long long total = 0, chunks = 0;
   for (int k = 0; k < count; ++k) {
     const pdes_mt_tensor& t = tensors[k];
     if (t.n < 0 || t.n >= MT_LONGEST - total || t.block0 < 0 || t.cls < 0 || t.cls >= nclasses) return PDES_EINVAL;
@@ -633,11 +823,15 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     if (params[k] % size || grads[k] % size) return PDES_EALIGN;
     total += t.n;
   }
-  hipStream_t st = static_cast<hipStream_t>(stream);
   StepArgs a;
+  a.tiles = tiles_of(s.bits, size, total);
+  const long long chunk = (long long)a.tiles * MT_TILE;
+  for (int k = 0; k < count; ++k) chunks += (tensors[k].n + chunk - 1) / chunk;
+  if (chunks >= 1ll << 24) return PDES_ENOSUP;             // (a launch has under 2^32 threads)
+  hipStream_t st = static_cast<hipStream_t>(stream);
   if (captured) {
     ClassArgs ca;
-    ca.n = nclasses; ca.seed = s.seed; ca.out = static_cast<MtHyper*>(s.hyper);
+    ca.n = nclasses; ca.maximize = s.maximize; ca.seed = s.seed; ca.out = static_cast<MtHyper*>(s.hyper);
     for (int k = 0; k < nclasses; ++k) {
       ca.lr[k] = classes[k].lr; ca.b1[k] = classes[k].beta1; ca.b2[k] = classes[k].beta2;
       ca.eps[k] = classes[k].eps; ca.wd[k] = classes[k].weight_decay;
@@ -647,15 +841,21 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     PDES_LAUNCH_CHECK();
   } else {
     for (int k = 0; k < nclasses; ++k)
-      a.h[k] = constants(classes[k].lr, classes[k].beta1, classes[k].beta2, classes[k].eps, classes[k].weight_decay, classes[k].step, s.seed);
+      a.h[k] = constants(classes[k].lr, classes[k].beta1, classes[k].beta2, classes[k].eps, classes[k].weight_decay, s.maximize != 0, classes[k].step, s.seed);
   }
   a.hdev = captured ? static_cast<const MtHyper*>(s.hyper) : nullptr;
-  a.partials = s.norm_rows; a.norm_out = s.norm_out;
+  const bool clip = s.norm_rows != nullptr;
+  const long long bytes = total * (2 * size + (s.low ? 2 : 0) + (s.bits == 32 ? 8 : 2));
+  a.rows = s.norm_rows; a.norm = clip ? s.norm_out : nullptr;
   a.m = s.exp_avg; a.v = s.exp_avg_sq; a.ms = s.exp_avg_scale; a.rs = s.rms_scale; a.low = s.low;
-  a.limit = s.limit; a.sign = s.maximize ? -1.f : 1.f;
-  // small lists are cut finely so that every CU has work; long ones into chunks that make the look-up disappear
-  a.tiles = total < (8ll << 20) ? 1 : 4;
-  const long long chunk = (long long)a.tiles * MT_TILE;
+  a.limit = s.limit;
+  if (clip && total > LONG_LIST) {
+    // every workgroup of a step can add up the rows by itself, which saves a launch (1 M elements with 8-bit states: 10.6 us for
+    // norm and step, 13.5 with the launch); where they are many, that costs more (64 M: 219 us, 210 with the launch)
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(MT_ROWS), 0, st, a.rows, a.norm);
+    PDES_LAUNCH_CHECK();
+    a.rows = nullptr;
+  }
   for (int done = 0; done < count;) {
     int k = 0;
     a.chunks = 0;
@@ -669,11 +869,10 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     }
     for (; k < MT_MAX; ++k) a.chunk0[k] = 0xffffffffu;
     if (a.chunks == 0) continue;
-    const unsigned grid = a.chunks < 2048 ? a.chunks : 2048;
-    if (s.dtype == PDES_MT_F32) launch_step<F32, false>(s.bits, a, grid, st);
-    else if (s.dtype == PDES_MT_F16) launch_step<F16, false>(s.bits, a, grid, st);
-    else if (s.low) launch_step<BF16, true>(s.bits, a, grid, st);
-    else launch_step<BF16, false>(s.bits, a, grid, st);
+    if (s.dtype == PDES_MT_F32) launch_step<F32, false>(s.bits, bytes, a, st);
+    else if (s.dtype == PDES_MT_F16) launch_step<F16, false>(s.bits, bytes, a, st);
+    else if (s.low) launch_step<BF16, true>(s.bits, bytes, a, st);
+    else launch_step<BF16, false>(s.bits, bytes, a, st);
     PDES_LAUNCH_CHECK();
   }
   return PDES_OK;

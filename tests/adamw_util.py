@@ -73,14 +73,16 @@ def dither(seed, t, ordinal, blocks):
 
 
 def held(x, noise, root):
-    """(codes as uint8, scales) of fp32 rows x [blocks, 256], non-finite values included, from the definition in fp32"""
+    """(codes as uint8, scales) of fp32 rows x [blocks, 256], non-finite values included, from the definition in fp32: x times 448 /
+    largest, cut to multiples of 2^-29 under 2^-6 (2^-20 of a spacing there), plus the noise, rounded down"""
     mag = np.abs(x)
     fine = np.isfinite(x)
     top = np.where(fine, mag, np.float32(0)).max(1, keepdims=True)
     live = top >= np.float32(2.0 ** -100)
     with np.errstate(all='ignore'):
         inverse = np.where(live, np.float32(448) / top, np.float32(0)).astype(np.float32)
-        y = (np.where(fine, mag, np.float32(0)) * inverse).astype(np.float32)
+        y = np.minimum((np.where(fine, mag, np.float32(0)) * inverse).astype(np.float32), np.float32(448))
+        y = np.where(y < 2.0 ** -6, np.floor(y * np.float32(2.0 ** 29)) * np.float32(2.0 ** -29), y).astype(np.float32)
         y = (y * np.float32(2.0 ** -120)).astype(np.float32)
     code = np.minimum((y.view(np.int32).astype(np.int64) + noise) >> 20, 0x7e)
     if root:
@@ -100,8 +102,8 @@ def rows(x, n):
 
 
 def step8(w, g, mq, ms, rq, rs, t, lr, betas, eps, wd, seed, ordinal, factor=np.float32(1)):
-    """one step with 8-bit states in fp32, one rounding per operation: (w, m codes, m scales, r codes, r scales).  mq / rq:
-    the held values [blocks, 256] as fp32; w, g fp32 [n]"""
+    """one step with 8-bit states in fp32, one rounding per operation: (w, its change by the gradient, m codes, m scales, r codes,
+    r scales).  mq / rq: the held values [blocks, 256] as fp32; w, g fp32 [n]"""
     f = np.float32
     b1, b2 = betas
     n = w.size
@@ -113,6 +115,7 @@ def step8(w, g, mq, ms, rq, rs, t, lr, betas, eps, wd, seed, ordinal, factor=np.
         for_m, for_r = dither(seed, t, ordinal, m.shape[0])
         out = held(m, for_m, False) + held(r, for_r, True)
         u = m / (r * f(1 / math.sqrt(1 - b2 ** t)) + f(eps))
-        new = rows(w, n) * f(1 - lr * wd) - u * f(lr / (1 - b1 ** t))
+        change = u * f(lr / (1 - b1 ** t))
+        new = rows(w, n) * f(1 - lr * wd) - change
     assert new.dtype == np.float32
-    return (new.reshape(-1)[:n],) + out
+    return (new.reshape(-1)[:n], change.reshape(-1)[:n]) + out
