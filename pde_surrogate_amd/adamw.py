@@ -190,7 +190,9 @@ class _Launch:
 
     def __init__(self, arena, members, classes):
         # members: (parameter, its class, block0, ordinal); classes: (param_group, step tensor)
-        self.arena, self.classes, self.count = arena, classes, len(members)
+        self.arena, self.count = arena, len(members)
+        # on the host, counts are incremented through numpy: a tenth of the time of a tensor's addition
+        self.classes = [(g, step, None if step.is_cuda else step.numpy()) for g, step in classes]
         self.params = [m[0] for m in members]
         self.table = (AdamWClass * len(classes))()
         self.state = st = AdamWState()
@@ -299,7 +301,7 @@ class FusedAdamW(torch.optim.Optimizer):
     # -- states ----------------------------------------------------------------------------------------------------------
     def _make_states(self, params):
         """states of parameters that have none, or have some from elsewhere (a loaded or copied state): one arena per type"""
-        by_type, steps = {}, {}
+        by_type, steps, to, source = {}, {}, [], []
         for p in params:
             by_type.setdefault(p.dtype, []).append(p)
         for dtype, ps in by_type.items():
@@ -316,13 +318,17 @@ class FusedAdamW(torch.optim.Optimizer):
                         old = had[name]
                         if tuple(old.shape) != tuple(view.shape):
                             raise ValueError(f'state {name!r} has shape {tuple(old.shape)}, the parameter needs {tuple(view.shape)}')
-                        view.copy_(old)
+                        to.append(view)
+                        source.append(old)
                 count = float(had['step']) if had else 0.0
                 if count not in steps:
                     steps[count] = torch.tensor(count, dtype=torch.float32, device=self._device if self.capturable else 'cpu')
                 self.state[p] = {'step': steps[count], **mine}
                 self._where[p] = (arena, block0)
                 block0 += -(-p.numel() // BLOCK)
+        if to:
+            with torch.no_grad():
+                torch._foreach_copy_(to, source)
 
     def flat_state(self):
         """{name: [the flat buffers that hold this state, one per element type]}: the parameters' states one behind the other
@@ -486,7 +492,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if self.capturable:
                 hyper = torch.empty(_HYPER_BYTES, dtype=torch.uint8, device=device)
                 st.hyper = hyper.data_ptr()
-            for c, (g, step) in zip(x.table, x.classes):
+            for c, (g, step, count) in zip(x.table, x.classes):
                 lr = g['lr']
                 c.beta1, c.beta2 = g['betas']
                 c.eps, c.weight_decay = g['eps'], g['weight_decay']
@@ -495,8 +501,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     c.lr_dev = lr.data_ptr() if isinstance(lr, torch.Tensor) else None
                     c.lr = 0.0 if isinstance(lr, torch.Tensor) else lr
                 else:
-                    step += 1
-                    c.step, c.lr = int(step), lr
+                    count += 1
+                    c.step, c.lr = int(count), lr
             rc = L.pdes_adamw_step(x.ptr_at, x.grad_at, x.tensor_at, x.count, x.table, len(x.classes), ctypes.byref(st), stream)
             _lib.check(rc, 'pdes_adamw_step')
             host.changed(x.params, False)

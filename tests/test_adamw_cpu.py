@@ -142,3 +142,19 @@ def test_held_values_are_within_a_spacing_and_right_on_average():
     big = np.abs(x) > top * 2.0 ** -12                     # (smaller ones are held by chance alone)
     rel = (total / times - x)[big] / np.abs(x)[big]
     assert abs(rel.mean()) < 5e-4 and (np.abs(rel) < 5 * 0.0625 / math.sqrt(times) * np.maximum(1, 2.0 ** -6 * top.repeat(256, 1)[big] / 448 * 448 / np.abs(x)[big] * 8)).mean() > 0.99
+
+
+def test_cli_flags(tmp_path):
+    """--optimizer and --clip-norm belong to --mode dropin; refused before a directory is made"""
+    import train_codec_max_likelihood as m
+    import train_codec_mixed_residual as t
+    for cli in (t, m):
+        a = cli.Parser().parse(['--exp-dir', str(tmp_path / 'ok'), '--mode', 'dropin', '--optimizer', 'adamw8', '--clip-norm', '0.5'])
+        assert (a.optimizer, a.clip_norm) == ('adamw8', 0.5)
+        a = cli.Parser().parse(['--exp-dir', str(tmp_path / 'ok')])
+        assert (a.optimizer, a.clip_norm) == ('adam', None)
+        for argv in (['--optimizer', 'adamw'], ['--clip-norm', '1'], ['--mode', 'dropin', '--clip-norm', '-1'],
+                     ['--mode', 'dropin', '--clip-norm', 'nan'], ['--mode', 'dropin', '--optimizer', 'sgd']):
+            with pytest.raises(SystemExit):
+                cli.Parser().parse(['--exp-dir', str(tmp_path / 'no')] + argv)
+    assert not (tmp_path / 'no').exists()

@@ -717,3 +717,58 @@ def test_refusals(dev):
         optim.clip_grad_norm_([p], 1.0, 1.0)
     with pytest.raises(ValueError, match='negative'):
         optim.clip_grad_norm_([p], -1.0)
+
+
+@pytest.mark.parametrize('optimizer,clip', [('adam', '0.5'), ('adamw', None), ('adamw', '0.5'), ('adamw8', '0.5')])
+def test_cli_runs(dev, tmp_path, monkeypatch, optimizer, clip):
+    """the training script with each optimiser: it runs, writes its files and the loss is finite"""
+    import json
+    import train_codec_mixed_residual as t
+    from pde_surrogate_amd import optim
+    monkeypatch.setenv('WORLD_SIZE', '1')
+    calls = []
+    for name, cls in (('Adam', optim.Adam), ('FusedAdamW', optim.FusedAdamW)):
+        real = cls.step
+        monkeypatch.setattr(cls, 'step', lambda self, *a, _r=real, _n=name, **k: (calls.append(_n), _r(self, *a, **k))[1])
+    argv = ['--exp-dir', str(tmp_path), '--ntrain', '32', '--ntest', '16', '--batch-size', '8', '--test-batch-size', '8', '--epochs', '2',
+            '--ckpt-freq', '2', '--cuda', '0', '--synthetic', '--blocks', '111', '--growth-rate', '8', '--init-features', '16',
+            '--weight-decay', '0.01', '--mode', 'dropin', '--optimizer', optimizer] + (['--clip-norm', clip] if clip else [])
+    with contextlib.redirect_stdout(io.StringIO()):
+        t.main(argv)
+    run = tmp_path / 'codec/mixed_residual/grf_kle512_ntrain32_run1_bs8_lr0.001_epochs2'
+    lt = np.loadtxt(run / 'training/loss_train.txt')
+    assert lt.shape == (2,) and np.isfinite(lt).all()
+    assert json.load(open(run / 'args.txt'))['optimizer'] == optimizer
+    assert calls == ['Adam' if optimizer == 'adam' else 'FusedAdamW'] * 8
+
+
+def test_the_flat_adam_of_a_network_goes_on_after_clipping(dev, monkeypatch):
+    """clip_grad_norm_ works in place on the views that the network's backward returned: optim.Adam still takes its one-launch step,
+    and equals torch.optim.Adam fed the clipped gradients"""
+    from pde_surrogate_amd import _lib, optim
+    from pde_surrogate_amd.models.codec import DenseED
+    torch.manual_seed(2)
+    with contextlib.redirect_stdout(io.StringIO()):
+        net = DenseED(1, 3, 32, [1, 1, 1], growth_rate=8, init_features=16).to(dev)
+    opt = optim.Adam(net.parameters(), lr=1e-3)
+    L, count = _lib.lib(), []
+    real = L.pdes_adam_step_host
+
+    class Spy:
+        def __getattr__(self, k):
+            if k == 'pdes_adam_step_host':
+                count.append(1)
+                return real
+            return getattr(L, k)
+    monkeypatch.setattr(_lib, '_lib', Spy())
+    for t in range(3):
+        net.zero_grad()
+        net(torch.rand(4, 1, 32, 32, device=dev)).square().mean().backward()
+        before = [p.grad.clone() for p in net.parameters()]
+        norm = optim.clip_grad_norm_(net.parameters(), 1e-3)
+        want = math.sqrt(sum(float((au.f64(g) ** 2).sum()) for g in before))
+        assert want > 1e-3 and abs(float(norm) / want - 1) <= 1.001 * au.U
+        for p, g in zip(net.parameters(), before):
+            au.within(p.grad, au.f64(g) * 1e-3 / (want + 1e-6), np.abs(au.f64(g)) * 1e-3 / want * 6 * au.U + au.TINY, 'clipped')
+        opt.step()
+    assert len(count) == 3

@@ -6,7 +6,8 @@ loop body of :197-211 (F.mse_loss, one-cycle LR, Adam) and the test() of :166-19
                            trainer with pdes_mse_loss as the loss launch (device-resident data, flat Adam kernel,
                            RCCL all-reduce under torchrun);
   --mode dropin            the reference's loop body verbatim on the drop-in modules (model(input),
-                           pde_surrogate_amd.metrics.mse_loss, loss.backward(), torch.optim.Adam).
+                           pde_surrogate_amd.metrics.mse_loss, loss.backward(), torch.optim.Adam; --optimizer and
+                           --clip-norm as in train_codec_mixed_residual.py).
 
 The loss needs output data: `--synthetic` is not available here; datasets are the reference's HDF5 files (or .npz
 files with the same stem holding `input` and `output`).
@@ -16,8 +17,6 @@ import time
 
 import numpy as np
 import torch
-from pde_surrogate_amd import optim          # the reference's `import torch.optim as optim`, redirected
-
 from pde_surrogate_amd import parallel
 from pde_surrogate_amd.metrics import TestMetrics, mse_launch, mse_loss
 from pde_surrogate_amd.models.codec import DenseED
@@ -92,7 +91,7 @@ def main(argv=None):
     else:
         if world > 1:
             raise SystemExit('--mode dropin is the single-GPU reference loop; use --mode fused with torchrun')
-        optimizer = optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay)
+        optimizer, clip = _mr.make_optimizer(args, model)
 
     logger = {'loss_train': [], 'loss_test': [], 'r2_test': [], 'nrmse_test': []}
     metrics = TestMetrics(3, device)
@@ -148,6 +147,7 @@ def main(argv=None):
                 step = (epoch - 1) * len(train_loader) + batch_idx
                 lr = scheduler.step(step / total_steps)
                 adjust_learning_rate(optimizer, lr)
+                clip()
                 optimizer.step()
                 loss_train += loss.item()
             loss_train /= batch_idx

@@ -13,7 +13,9 @@ HIP kernels (pde_surrogate_amd).  Two loop bodies are available:
 
 Additive flags (not in the reference): --mode, --graph, --synthetic (generate GRF-KLE /
 channelized inputs instead of reading the HDF5 files, which are not redistributed; R^2 / NRMSE need
-the FEniCS targets of the real files and are reported as nan in that mode).
+the FEniCS targets of the real files and are reported as nan in that mode); with --mode dropin also
+--optimizer adamw | adamw8 (decoupled weight decay, moments in 32 or 8 bits, optim.FusedAdamW) and
+--clip-norm (gradients clipped by their common norm before the step).
 
     python train_codec_mixed_residual.py --data grf_kle512 --ntrain 4096 --batch-size 32 --synthetic
     python -m torch.distributed.run --nproc-per-node 8 --master-addr 127.0.0.1 \\
@@ -69,6 +71,10 @@ def validate_args(args, world):
     DenseED itself, in the reference too: one stride-2 convolution per encoding stage (codec.py:242, :113-118) and one
     x2 upsampling per decoding stage give an output of the input's size -- which the loss needs (darcy.py:172-176
     multiplies input and output fields) -- only when imsize is a multiple of 2^(1 + encoding blocks)."""
+    if args.mode != 'dropin' and (args.optimizer != 'adam' or args.clip_norm is not None):
+        raise SystemExit('--optimizer and --clip-norm are options of --mode dropin (the fused step holds Adam)')
+    if args.clip_norm is not None and not args.clip_norm >= 0.0:
+        raise SystemExit(f'--clip-norm {args.clip_norm} must not be negative')
     down = 2 ** (1 + len(args.blocks) // 2)
     if args.imsize < down or args.imsize % down:
         raise SystemExit(f'--imsize {args.imsize}: DenseED with blocks {args.blocks} halves the field {len(args.blocks) // 2 + 1} '
@@ -104,6 +110,9 @@ class Parser(argparse.ArgumentParser):
         self.add_argument('--no-graph', action='store_true', default=False, help='(default; kept for older scripts)')
         self.add_argument('--synthetic', action='store_true', default=False,
                           help='generate inputs instead of reading HDF5 files')
+        self.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'adamw', 'adamw8'],
+                          help='dropin mode: Adam, or AdamW with 32-bit or 8-bit moments')
+        self.add_argument('--clip-norm', type=float, default=None, help='dropin mode: clip the gradients to this norm')
 
     def parse(self, argv=None, rank=0, world=1):
         """rank / world: under torchrun every rank parses, only rank 0 creates directories, prints and writes args.txt"""
@@ -133,6 +142,18 @@ class Parser(argparse.ArgumentParser):
             with open(args.run_dir + "/args.txt", 'w') as args_file:
                 json.dump(vars(args), args_file, indent=4)
         return args
+
+
+def make_optimizer(args, model):
+    """(optimiser of --mode dropin, what to do between loss.backward() and its step)"""
+    if args.optimizer == 'adam':
+        adam = optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay)
+        if args.clip_norm is None:
+            return adam, lambda: None
+        return adam, lambda: optim.clip_grad_norm_(model.parameters(), args.clip_norm)
+    # clips as it reads the gradients
+    return optim.FusedAdamW(model.parameters(), lr=args.lr, weight_decay=args.weight_decay, clip_norm=args.clip_norm,
+                            state_bits=8 if args.optimizer == 'adamw8' else 32, seed=args.seed & 0xffffffff), lambda: None
 
 
 def dataset_files(args):
@@ -224,7 +245,7 @@ def main(argv=None):
     else:
         if world > 1:
             raise SystemExit('--mode dropin is the single-GPU reference loop; use --mode fused with torchrun')
-        optimizer = optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay)
+        optimizer, clip = make_optimizer(args, model)
 
     logger = {'loss_train': [], 'loss_test': [], 'r2_test': [], 'nrmse_test': []}
 
@@ -298,6 +319,7 @@ def main(argv=None):
                 step = (epoch - 1) * len(train_loader) + batch_idx
                 lr = scheduler.step(step / total_steps)
                 adjust_learning_rate(optimizer, lr)
+                clip()
                 optimizer.step()
                 loss_train += loss.item()
             loss_train /= batch_idx
