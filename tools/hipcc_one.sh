@@ -3,8 +3,9 @@
 #   bash tools/hipcc_one.sh conv_mfma_wgrad wgrad_kernelILi3E
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 SRC=$ROOT/pde_surrogate_amd/csrc/$1.hip
+EXTRA=$(cd $ROOT && python3 -c "from pde_surrogate_amd.build import FILE_FLAGS as f; print(*f.get('$1.hip', []))")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast -Wno-unused-result -munsafe-fp-atomics \
-  $PDES_EXTRA_FLAGS -Rpass-analysis=kernel-resource-usage -c $SRC -o $ROOT/pde_surrogate_amd/csrc/$1.o > /tmp/hipcc_one.log 2>&1
+  $EXTRA $PDES_EXTRA_FLAGS -Rpass-analysis=kernel-resource-usage -c $SRC -o $ROOT/pde_surrogate_amd/csrc/$1.o > /tmp/hipcc_one.log 2>&1
 rc=$?
 grep -E "error|warning: v" -A6 /tmp/hipcc_one.log | head -40
 python3 - "$2" <<'PY'
