@@ -83,10 +83,14 @@ def _check_tensor(t, what):
                            'move tensors to cuda)')
 
 
-def _repeated(pairs):
-    """whether one of the (address, size) pairs with elements appears twice"""
-    used = [x for x, n in pairs if n]
-    return len(set(used)) < len(used)
+def _overlap(stretches):
+    """whether two of the (address, bytes) stretches have bytes in common"""
+    end = 0
+    for start, size in sorted(x for x in stretches if x[1]):
+        if start < end:
+            return True
+        end = start + size
+    return False
 
 
 def _words(n):
@@ -108,7 +112,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """torch.nn.utils.clip_grad_norm_ for parameters on one GPU: returns the norm of all gradients taken as one vector (0-d
     fp32 on the device) and multiplies the gradients in place by min(1, max_norm / (norm + 1e-6)), without synchronising.
     norm_type is 2 (summed in fp64) or infinity.  max_norm = inf finds the norm only.  Where the factor is 1 the gradients
-    are read once and not written.  A gradient that is not dense (an expanded one) or appears twice is refused.
+    are read once and not written.  A gradient that is not dense (an expanded one) or shares memory with another is refused.
     error_if_nonfinite waits for the norm and raises, with the gradients as they were, if it is not finite."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, norm_type = float(max_norm), float(norm_type)
@@ -118,15 +122,15 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError(f'clip_grad_norm_: max_norm {max_norm} must not be negative')
     n = len(params)
     (ptrs, ptr_at), (sizes, size_at) = _words(3 * n), _words(3 * n)
-    *counts, index, bad, twice = _host().gradients(params, ptr_at, size_at)
+    *counts, index, bad, shared = _host().gradients(params, ptr_at, size_at)
     if bad >= 0:
         g = params[bad].grad
         _check_tensor(g, 'a gradient')
         if not _dense(g):
             raise RuntimeError('clip_grad_norm_: a gradient is not dense')
         raise RuntimeError(f'clip_grad_norm_: gradients on cuda:{index} and {g.device}')
-    if twice:
-        raise ValueError('clip_grad_norm_: a gradient appears twice')
+    if shared:
+        raise ValueError('clip_grad_norm_: two gradients share their memory')
     lists = [(dtype, ptr_at + 8 * n * dtype, size_at + 8 * n * dtype, count) for dtype, count in enumerate(counts) if count]
     if not lists:
         return torch.tensor(0.0)
@@ -151,6 +155,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
                 clip(*x, max_norm)
             _host().changed(params, True)
     return norm
+
+
+def _check_lr(lr, device):
+    if lr.dim() or lr.dtype != torch.float32 or lr.device != device:
+        raise ValueError(f'lr as a tensor has to be a 0-d float32 tensor on {device}, got {lr.dim()}-d {lr.dtype} on {lr.device}')
 
 
 class _Arena:
@@ -234,8 +243,12 @@ class FusedAdamW(torch.optim.Optimizer):
     seed            of the stochastic rounding: equal seeds, parameters and gradients give equal bits.
 
     A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
-    dense.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse and complex parameters are
-    not offered.  A gradient that is not finite spoils the elements it belongs to and no others."""
+    dense, and no two may share memory.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse
+    and complex parameters are not offered.  A gradient that is not finite spoils the elements it belongs to and no others.
+    With 8-bit states eps under 2^-100 counts as 2^-100, and blocks whose largest value is under that are held as zeros.
+
+    A graph captured from a step holds the states it was captured with: capture again after load_state_dict, and after a step
+    in which other parameters had gradients.  Memory that such a graph may write to is kept for as long as the optimiser."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
                  clip_norm=None, maximize=False, capturable=False, seed=0):
@@ -276,9 +289,10 @@ class FusedAdamW(torch.optim.Optimizer):
     def _check_group(self, group):
         device = self._device
         lr, (b1, b2) = group['lr'], group['betas']
-        if isinstance(lr, torch.Tensor) and not (self.capturable and lr.is_cuda and lr.dim() == 0 and lr.dtype == torch.float32):
-            raise ValueError('lr as a tensor has to be a 0-d float32 device tensor of an optimiser with capturable=True')
-        if not isinstance(lr, torch.Tensor) and not 0.0 <= lr:
+        if isinstance(lr, torch.Tensor):
+            if not self.capturable:
+                raise ValueError('lr as a tensor needs an optimiser with capturable=True')
+        elif not 0.0 <= lr:
             raise ValueError(f'Invalid learning rate: {lr}')
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f'Invalid betas: {group["betas"]}')
@@ -296,6 +310,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise ValueError(f'parameters on {device} and {p.device}')
         if len({id(p) for p in group['params']}) < len(group['params']):
             raise ValueError('a parameter appears twice')
+        if isinstance(lr, torch.Tensor):
+            _check_lr(lr, device)
         self._device = device
 
     # -- states ----------------------------------------------------------------------------------------------------------
@@ -388,7 +404,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if self._where and not any('step' in self.state.get(p, ()) for p in self._where):
             self._retire(self._arenas)
             self._reset()                  # the program has emptied the states, or put others in their place
-        if _repeated((p.data_ptr(), p.numel()) for _, p, _ in active):
+        if _overlap([(p.data_ptr(), p.numel() * p.element_size()) for _, p, _ in active]):
             raise RuntimeError('FusedAdamW: two parameters share their memory')
         new = [p for _, p, _ in active if p not in self._where or 'step' not in self.state.get(p, ())]
         if new:
@@ -453,6 +469,8 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self._device is None:                                # (groups without parameters)
+            return loss
         with _lib.device_guard(self._device):
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
@@ -498,13 +516,18 @@ class FusedAdamW(torch.optim.Optimizer):
                 c.eps, c.weight_decay = g['eps'], g['weight_decay']
                 if self.capturable:
                     c.step_dev = step.data_ptr()
-                    c.lr_dev = lr.data_ptr() if isinstance(lr, torch.Tensor) else None
-                    c.lr = 0.0 if isinstance(lr, torch.Tensor) else lr
+                    if isinstance(lr, torch.Tensor):
+                        _check_lr(lr, device)
+                        c.lr_dev, c.lr = lr.data_ptr(), 0.0
+                    else:
+                        c.lr_dev, c.lr = None, lr
                 else:
-                    count += 1
-                    c.step, c.lr = int(count), lr
+                    c.step, c.lr = int(count) + 1, lr
             rc = L.pdes_adamw_step(x.ptr_at, x.grad_at, x.tensor_at, x.count, x.table, len(x.classes), ctypes.byref(st), stream)
             _lib.check(rc, 'pdes_adamw_step')
+            if not self.capturable:
+                for _, _, count in x.classes:
+                    count += 1
             host.changed(x.params, False)
             if x.arena.stream != current and not capturing:     # freed later than this stream's work on them
                 for buf in x.arena.bufs.values():

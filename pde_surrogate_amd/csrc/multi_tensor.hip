@@ -639,14 +639,15 @@ struct ClassArgs {
   float* step_dev[MT_CLASSES];
   MtHyper* out;
   uint32_t seed;
-  int n, maximize;
+  int n, maximize, bits;
 };
-__host__ __device__ __forceinline__ MtHyper constants(double lr, double b1, double b2, double eps, double wd, bool maximize, long long t, uint32_t seed) {
+__host__ __device__ __forceinline__ MtHyper constants(double lr, double b1, double b2, double eps, double wd, bool maximize, int bits, long long t,
+                                                       uint32_t seed) {
   MtHyper h;
   h.decay = (float)(1.0 - lr * wd);
   h.step = (float)(lr / (1.0 - pow(b1, (double)t)));
   h.rc2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
-  h.eps = (float)eps;
+  h.eps = (float)(bits == 8 && eps < 0x1p-100 ? 0x1p-100 : eps);      // (r under 2^-100 is held as zero)
   h.b1 = (float)b1;
   h.ob1 = (float)(maximize ? b1 - 1.0 : 1.0 - b1);           // (of the gradient, only its sign in m differs)
   h.b2 = (float)b2; h.ob2 = (float)(1.0 - b2);
@@ -658,7 +659,7 @@ __global__ __launch_bounds__(64) void adamw_count_kernel(const ClassArgs a) {
   if (k >= a.n) return;
   const float t = *a.step_dev[k] + 1.f;
   *a.step_dev[k] = t;
-  a.out[k] = constants(a.lr_dev[k] ? (double)*a.lr_dev[k] : a.lr[k], a.b1[k], a.b2[k], a.eps[k], a.wd[k], a.maximize, (long long)t, a.seed);
+  a.out[k] = constants(a.lr_dev[k] ? (double)*a.lr_dev[k] : a.lr[k], a.b1[k], a.b2[k], a.eps[k], a.wd[k], a.maximize, a.bits, (long long)t, a.seed);
 }
 
 constexpr long long LONG_LIST = 8ll << 20;
@@ -831,7 +832,7 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (captured) {
     ClassArgs ca;
-    ca.n = nclasses; ca.maximize = s.maximize; ca.seed = s.seed; ca.out = static_cast<MtHyper*>(s.hyper);
+    ca.n = nclasses; ca.maximize = s.maximize; ca.bits = s.bits; ca.seed = s.seed; ca.out = static_cast<MtHyper*>(s.hyper);
     for (int k = 0; k < nclasses; ++k) {
       ca.lr[k] = classes[k].lr; ca.b1[k] = classes[k].beta1; ca.b2[k] = classes[k].beta2;
       ca.eps[k] = classes[k].eps; ca.wd[k] = classes[k].weight_decay;
@@ -841,7 +842,8 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     PDES_LAUNCH_CHECK();
   } else {
     for (int k = 0; k < nclasses; ++k)
-      a.h[k] = constants(classes[k].lr, classes[k].beta1, classes[k].beta2, classes[k].eps, classes[k].weight_decay, s.maximize != 0, classes[k].step, s.seed);
+      a.h[k] = constants(classes[k].lr, classes[k].beta1, classes[k].beta2, classes[k].eps, classes[k].weight_decay, s.maximize != 0, s.bits,
+                         classes[k].step, s.seed);
   }
   a.hdev = captured ? static_cast<const MtHyper*>(s.hyper) : nullptr;
   const bool clip = s.norm_rows != nullptr;

@@ -8,6 +8,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <algorithm>
+#include <utility>
 #include <vector>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -73,8 +74,8 @@ PyObject* gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // gradients(params, out, sizes) -> (count of float32, of bfloat16, of float16 gradients, their device, place of the first
-// parameter whose gradient is not a dense device tensor of one of these types on one device, or -1, whether a gradient with
-// elements appears twice).  out, sizes: addresses of arrays of three times the list's length, one third for each type
+// parameter whose gradient is not a dense device tensor of one of these types on one device, or -1, whether two gradients have
+// memory in common).  out, sizes: addresses of arrays of three times the list's length, one third for each type
 PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 3 || !as_list(args[0])) {
@@ -98,14 +99,15 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       out[c * n + count[c]] = reinterpret_cast<unsigned long long>(g.data_ptr());
       sizes[c * n + count[c]++] = (unsigned long long)g.numel();
     }
-    std::vector<unsigned long long> used;
+    std::vector<std::pair<unsigned long long, unsigned long long>> used;         // first byte, byte behind the last
     used.reserve(n);
     for (int c = 0; c < 3; ++c)
       for (Py_ssize_t k = 0; k < count[c]; ++k)
-        if (sizes[c * n + k]) used.push_back(out[c * n + k]);
+        if (sizes[c * n + k]) used.emplace_back(out[c * n + k], out[c * n + k] + sizes[c * n + k] * (c == 0 ? 4 : 2));
     std::sort(used.begin(), used.end());
-    const bool twice = std::adjacent_find(used.begin(), used.end()) != used.end();
-    return Py_BuildValue("nnnini", count[0], count[1], count[2], device, bad, (int)twice);
+    bool shared = false;
+    for (size_t k = 1; k < used.size(); ++k) shared |= used[k].first < used[k - 1].second;
+    return Py_BuildValue("nnnini", count[0], count[1], count[2], device, bad, (int)shared);
   });
 }
 
