@@ -318,15 +318,12 @@ __device__ __forceinline__ float new_weight(float w, float m, float r, const MtH
   const float u = m / (r * h.rc2 + h.eps);
   return w * h.decay - u * h.step;
 }
-// The same in the 8-bit kernel, which computes about as long as it waits for memory.  A weight that is rounded to 16 bits takes the
-// quotient from the reciprocal instruction (off by a place, 2^-23, where the weight's rounding is 2^-9 or 2^-12); the fix-up
-// gives the quotients of zeros, infinities and NaN.
-template <class T, bool LOW>
-__device__ __forceinline__ float new_weight(float w, float m, float r, const MtHyper& h) {
-  if constexpr (sizeof(typename T::E) == 4 || LOW) return new_weight(w, m, r, h);
-  const float den = r * h.rc2 + h.eps;
+// The same in the 8-bit kernel for weights of 16 bits (see EXACT there): the quotient from the reciprocal instruction; the fix-up
+// gives the quotients of zeros, infinities and NaN
+__device__ __forceinline__ float new_weight_16(float w, float m, float r, const MtHyper& h) {
+  const float den = fmaf(r, h.rc2, h.eps);
   const float u = __builtin_amdgcn_div_fixupf(m * __builtin_amdgcn_rcpf(den), den, m);
-  return w * h.decay - u * h.step;
+  return fmaf(-u, h.step, w * h.decay);
 }
 
 // what clipping multiplies the gradients by
@@ -461,7 +458,14 @@ __device__ __forceinline__ float root(float x) {
   float r = fmaf(-under, s, x) <= 0.f ? under : s;
   return fmaf(-over, s, x) > 0.f ? over : r;
 }
-constexpr int SUBNORMAL = 0x90;              // class mask: subnormal numbers of either sign
+// The same but for one in two million x, where the result is the neighbour: from the reciprocal root (off by a place) and one
+// correction by the residual, whose own error is 2^-22 of a place.  Not for infinity and subnormal numbers.
+__device__ __forceinline__ float near_root(float x) {
+  const int bits = __float_as_int(x), least = 0x00800000;                      // (2^-126; x is not negative)
+  const float y = __builtin_amdgcn_rsqf(__int_as_float(bits > least ? bits : least)), s = x * y;
+  return fmaf(fmaf(-s, s, x), 0.5f * y, s);
+}
+constexpr int ODD_ROOT = 0x290;              // class mask: subnormal numbers and infinity
 
 // A half wave holds a block, a lane eight elements of it: consecutive ones of 16 bits, or twice four of 32 bits, 128 elements
 // apart, so that each access of a wave covers whole lines (332 M fp32 parameters, streaming: 852 us; eight consecutive ones, two
@@ -513,6 +517,10 @@ __device__ __forceinline__ void put_codes(uint8_t* q, u32x2 w) {
 template <class T, bool LOW, bool CLIP, bool NT, bool ALL>
 __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, uint8_t* mq, uint8_t* rq, float* ms, float* rs, int16_t* low,
                                       long long cnt, float gf, const MtHyper& h, uint32_t key, int lane) {
+  // Weights of 16 bits leave 10 bytes of traffic per element, about the time of this arithmetic.  There the weight itself is
+  // computed with fused sums and the reciprocal instruction, off by a few places of 2^-24 before it is rounded by 2^-9 or 2^-12.
+  // The moments are always held to the last place: which of two codes a value gets depends on it, and so do later scales.
+  constexpr bool EXACT = sizeof(typename T::E) == 4 || LOW;
   typename T::E pe[8], ge[8];
   int16_t lw[8] = {};
   load8<T, ALL, NT>(p, cnt, pe);
@@ -533,8 +541,8 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
     const float gk = CLIP ? T::up(ge[k]) * gf : T::up(ge[k]);
     m[k] = m[k] * h.b1 + gk * h.ob1;
     v[k] = r[k] * r[k] * h.b2 + gk * gk * h.ob2;
-    r[k] = root(v[k]);
-    small |= __builtin_amdgcn_classf(v[k], SUBNORMAL);
+    r[k] = EXACT ? root(v[k]) : near_root(v[k]);
+    small |= __builtin_amdgcn_classf(v[k], ODD_ROOT);
   }
   if (small) {
 #pragma unroll
@@ -543,7 +551,8 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
   uint32_t mtop = 0, rtop = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    pe[k] = narrow<T, LOW>(new_weight<T, LOW>(widen<T, LOW>(pe[k], lw[k]), m[k], r[k], h), lw[k]);
+    const float w = widen<T, LOW>(pe[k], lw[k]);
+    pe[k] = narrow<T, LOW>(EXACT ? new_weight(w, m[k], r[k], h) : new_weight_16(w, m[k], r[k], h), lw[k]);
     const uint32_t mb = __float_as_uint(m[k]) & 0x7fffffffu, rb = __float_as_uint(r[k]);
     mtop = mb > mtop ? mb : mtop;
     rtop = rb > rtop ? rb : rtop;              // (r is not negative; a NaN with the sign is the largest as well)
@@ -664,12 +673,13 @@ __global__ __launch_bounds__(64) void adamw_count_kernel(const ClassArgs a) {
 
 constexpr long long LONG_LIST = 8ll << 20;
 // Tiles of a workgroup.  One, so that the workgroups walk through memory side by side (332 M fp32 elements: 1,749 us, with four
-// 1,790; 8-bit states: 919 and 1,011) -- but 16-bit elements with 8-bit states, which take as long to compute as to load, save
-// the look-up and the table's loads by two from 8 M and four from 64 M elements on (bf16, 128 M: 238 / 231 / 228 us with 1 / 2 / 4;
-// 32 M: 59.9 / 59.4 / 61.9; 4 M: 11.3 / 12.0 / 13.1)
-static uint32_t tiles_of(int bits, int size, long long total) {
+// 1,790; 8-bit states: 919 and 1,011).  16-bit elements with 8-bit states, where a workgroup's start (table, keys, clipping factor)
+// weighs more: two from 8 M elements on, and four from 32 M on with clipping, whose factor each workgroup loads first (bf16 elements
+// with one / two / four: 332 M 587 / 570 / 620 us; 4 M 10.2 / 10.2 / 13; clipped, with the norm, 332 M 752 / 697 / 694, 150 M with
+// low halves 440 / 429 / 422, 16 M 47 / 43 / 44)
+static uint32_t tiles_of(int bits, int size, bool clip, long long total) {
   if (bits == 32 || size == 4 || total < LONG_LIST) return 1;
-  return total < 8 * LONG_LIST ? 2 : 4;
+  return clip && total >= 4 * LONG_LIST ? 4 : 2;
 }
 static int item_size(int dtype) { return dtype == PDES_MT_F32 ? 4 : 2; }
 
@@ -825,7 +835,8 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
     total += t.n;
   }
   StepArgs a;
-  a.tiles = tiles_of(s.bits, size, total);
+  const bool clip = s.norm_rows != nullptr;
+  a.tiles = tiles_of(s.bits, size, clip, total);
   const long long chunk = (long long)a.tiles * MT_TILE;
   for (int k = 0; k < count; ++k) chunks += (tensors[k].n + chunk - 1) / chunk;
   if (chunks >= 1ll << 24) return PDES_ENOSUP;             // (a launch has under 2^32 threads)
@@ -846,7 +857,6 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
                          classes[k].step, s.seed);
   }
   a.hdev = captured ? static_cast<const MtHyper*>(s.hyper) : nullptr;
-  const bool clip = s.norm_rows != nullptr;
   const long long bytes = total * (2 * size + (s.low ? 2 : 0) + (s.bits == 32 ? 8 : 2));
   a.rows = s.norm_rows; a.norm = clip ? s.norm_out : nullptr;
   a.m = s.exp_avg; a.v = s.exp_avg_sq; a.ms = s.exp_avg_scale; a.rs = s.rms_scale; a.low = s.low;
