@@ -198,15 +198,15 @@ class _Launch:
     """one pdes_adamw_step call: parameters of one arena in up to eight classes"""
 
     def __init__(self, arena, members, classes):
-        # members: (parameter, its class, block0, ordinal); classes: (param_group, step tensor)
+        # members: (parameter, its class, block0, ordinal, its state's order); classes: (param_group, step tensor)
         self.arena, self.count = arena, len(members)
         # on the host, counts are incremented through numpy: a tenth of the time of a tensor's addition
         self.classes = [(g, step, None if step.is_cuda else step.numpy()) for g, step in classes]
-        self.params = [m[0] for m in members]
+        self.params, self.like = [m[0] for m in members], [m[4] for m in members]
         self.table = (AdamWClass * len(classes))()
         self.state = st = AdamWState()
         self.tensors = array('q')                          # pdes_mt_tensor: n, block0, cls | ordinal << 32
-        for p, cls, block0, ordinal in members:
+        for p, cls, block0, ordinal, _ in members:
             self.tensors.extend((p.numel(), block0, cls | ordinal << 32))
         # filled anew by every step; the sizes are what the parameters are held to
         (self.ptrs, self.ptr_at), (self.grads, self.grad_at) = _words(self.count), _words(self.count)
@@ -219,12 +219,16 @@ class _Launch:
         st.blocks, st.dtype = arena.blocks, _DTYPES[arena.dtype]
 
 
+class _Reordered(Exception):
+    """a parameter's memory has another order than its state's"""
+
+
 class _Plan:
     """the launches of a step, for as long as the same parameters have gradients and the states are the same"""
 
-    def __init__(self, launches, idle, state, states, params):
-        self.launches, self.idle = launches, idle          # idle: parameters without a gradient
-        self.state, self.states, self.params = state, states, params
+    def __init__(self, launches, params, state):
+        self.launches, self.params, self.state, self.states = launches, params, state, len(state)
+        self.mask = bytes(p.grad is not None for p in params)
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -245,7 +249,8 @@ class FusedAdamW(torch.optim.Optimizer):
     A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
     dense, and no two may share memory.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse
     and complex parameters are not offered.  A gradient that is not finite spoils the elements it belongs to and no others.
-    With 8-bit states eps under 2^-100 counts as 2^-100, and blocks whose largest value is under that are held as zeros.
+    With 8-bit states eps under 2^-100 counts as 2^-100, and blocks whose largest value is under that are held as zeros; they
+    belong to stretches of the parameter's memory, so a parameter keeps the order of its dimensions there for good.
 
     A graph captured from a step holds the states it was captured with: capture again after load_state_dict, and after a step
     in which other parameters had gradients.  Memory that such a graph may write to is kept for as long as the optimiser."""
@@ -267,7 +272,7 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     def _reset(self):
-        self._where = {}            # parameter -> (arena, block0)
+        self._where = {}            # parameter -> (arena, block0, a tensor without memory of the parameter's shape and order then)
         self._arenas = []
         self._plan = None
 
@@ -304,6 +309,8 @@ class FusedAdamW(torch.optim.Optimizer):
             _check_tensor(p, 'a parameter')
             if not _dense(p):
                 raise ValueError('a parameter is not dense (its elements do not fill one stretch of memory)')
+            if self.master_weights and p.dtype == torch.float16:
+                raise ValueError('master_weights keeps the low halves of bfloat16 parameters; float16 ones have none')
             if device is None:
                 device = p.device
             elif p.device != device:
@@ -340,7 +347,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 if count not in steps:
                     steps[count] = torch.tensor(count, dtype=torch.float32, device=self._device if self.capturable else 'cpu')
                 self.state[p] = {'step': steps[count], **mine}
-                self._where[p] = (arena, block0)
+                self._where[p] = (arena, block0, torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device='meta'))
                 block0 += -(-p.numel() // BLOCK)
         if to:
             with torch.no_grad():
@@ -417,20 +424,20 @@ class FusedAdamW(torch.optim.Optimizer):
                 step = self.state.get(p, {}).get('step')
                 holders[id(step)] = holders.get(id(step), 0) + 1
         for g, p, k in active:
-            (arena, block0), step = self._where[p], self.state[p]['step']
+            (arena, block0, like), step = self._where[p], self.state[p]['step']
             value = values.get(id(step))
             if value is None:
                 value = values[id(step)] = id(step) if self.capturable else float(step)
             key = (id(arena), id(g), value)
             if key not in classes:
                 classes[key] = (arena, g, step, [])
-            classes[key][3].append((p, block0, k))
+            classes[key][3].append((p, block0, k, like))
         counted = {}
         for key, (arena, g, step, members) in classes.items():
             if not (self.capturable and holders[id(step)] == len(members)):
                 self._retire(step)
                 step = step.clone()
-            for p, _, _ in members:
+            for p, _, _, _ in members:
                 self.state[p]['step'] = step
             counted[key] = step
         launches = []
@@ -438,15 +445,16 @@ class FusedAdamW(torch.optim.Optimizer):
             keys = [k for k in classes if k[0] == id(arena)]
             for at in range(0, len(keys), _CLASSES):
                 part = keys[at:at + _CLASSES]
-                members = sorted(((p, c, b, o) for c, key in enumerate(part) for p, b, o in classes[key][3]), key=lambda m: m[3])
+                members = sorted(((p, c, b, o, like) for c, key in enumerate(part) for p, b, o, like in classes[key][3]), key=lambda m: m[3])
                 launches.append(_Launch(arena, members, [(classes[key][1], counted[key]) for key in part]))
-        self._plan = _Plan(launches, [p for _, p in every if p.grad is None], self.state, len(self.state), len(every))
+        self._plan = _Plan(launches, [p for _, p in every], self.state)
         return self._plan
 
     @torch.no_grad()
     def _gather_slowly(self, launch):
         """addresses of a launch whose tensors are not all plain: gradients of another memory order go through a copy (returned,
-        to be kept until the launch is enqueued), everything else that the kernels cannot take is an error"""
+        to be kept until the launch is enqueued), a parameter that has got another order itself needs its state in that order,
+        everything else that the kernels cannot take is an error"""
         kept = []
         for k, p in enumerate(launch.params):
             g, dtype = p.grad, launch.arena.dtype
@@ -458,6 +466,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise RuntimeError(f'FusedAdamW: a parameter or gradient is no longer a {dtype} tensor on {self._device}')
             if not _dense(p) or p.is_neg():
                 raise RuntimeError('FusedAdamW: a parameter is no longer dense')
+            if not _same_order(p, launch.like[k]):
+                raise _Reordered
             if g.is_neg() or not (_dense(g) and _same_order(p, g)):
                 g = torch.empty_like(p).copy_(g)
                 kept.append(g)
@@ -475,36 +485,54 @@ class FusedAdamW(torch.optim.Optimizer):
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
                 raise RuntimeError('FusedAdamW: a step is captured into a graph only with capturable=True')
-            self._run(self._plan if self._plan is not None and self._fits(self._plan) else self._build(capturing), capturing)
+            plan = self._plan if self._plan is not None and self._fits(self._plan) else self._build(capturing)
+            try:
+                kept = self._gather(plan)
+            except _Reordered:
+                self._reorder()
+                plan = self._build(capturing)
+                kept = self._gather(plan)
+            self._run(plan, capturing)
+            del kept
         return loss
 
+    def _gather(self, plan):
+        """the addresses of a step, checked; returns what has to live until they are used"""
+        kept, host = [], _host()
+        for x in plan.launches:
+            if host.gather(x.params, x.like, x.state.dtype, self._device.index, x.size_at, x.ptr_at, x.grad_at) != -1:
+                kept += self._gather_slowly(x)
+        return kept
+
+    def _reorder(self):
+        """states of parameters whose memory has got another order: 32-bit ones move into it, 8-bit ones (blocks of memory) cannot"""
+        if self.state_bits == 8:
+            raise RuntimeError('FusedAdamW: a parameter has another memory order than its 8-bit state')
+        for p in [p for p, (_, _, like) in self._where.items() if not _same_order(p, like)]:
+            self._retire(self._where.pop(p), self.state[p])
+
     def _fits(self, plan):
-        count = _host().with_gradient
         return (plan.state is self.state and plan.states == len(self.state) and
-                plan.params == sum(len(g['params']) for g in self.param_groups) and
-                all(count(x.params) == x.count for x in plan.launches) and count(plan.idle) == 0)
+                _host().fits([g['params'] for g in self.param_groups], plan.params, plan.mask))
 
     def _run(self, plan, capturing):
         device, L, host = self._device, _lib.lib(), _host()
         current = torch.cuda.current_stream(device)
         stream = current.cuda_stream
-        kept = []
-        for x in plan.launches:
-            if host.gather(x.params, x.state.dtype, device.index, x.size_at, x.ptr_at, x.grad_at) != -1:
-                kept += self._gather_slowly(x)
-        rows = None
+        rows, norm = None, None
         if self.clip_norm is not None:
             lists = [(x.state.dtype, x.grad_at, x.size_at, x.count) for x in plan.launches if x.total]
             if lists:
                 rows = _norm_rows(lists, 2, device, stream)
-                self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
+                norm = torch.empty((), dtype=torch.float32, device=device)
             else:
-                self.grad_norm = torch.zeros((), dtype=torch.float32, device=device)
+                norm = torch.zeros((), dtype=torch.float32, device=device)
+        self.grad_norm = norm
         for x in plan.launches:
             st = x.state
             st.bits, st.maximize, st.seed = self.state_bits, self.maximize, self.seed
             if rows is not None:
-                st.norm_rows, st.norm_out, st.limit = rows.data_ptr(), self.grad_norm.data_ptr(), self.clip_norm
+                st.norm_rows, st.norm_out, st.limit = rows.data_ptr(), norm.data_ptr(), self.clip_norm
             else:
                 st.norm_rows = None
             if self.capturable:

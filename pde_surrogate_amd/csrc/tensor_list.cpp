@@ -16,11 +16,17 @@ namespace {
 
 int code_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
 
-// element k of a's memory is element k of b's, both dense
-bool same_dense_order(const at::Tensor& a, const at::Tensor& b) {
+bool same_strides(const at::Tensor& a, const at::Tensor& b) {
+  if (a.dim() != b.dim()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+// element k of a's memory is element k of b's and of `like`'s, all of them dense
+bool same_dense_order(const at::Tensor& a, const at::Tensor& b, const at::Tensor& like) {
   if (a.is_neg() || b.is_neg()) return false;          // (a lazy negation: the memory holds something else)
-  if (a.is_contiguous() && b.is_contiguous()) return true;
-  return a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense() && a.strides() == b.strides();
+  if (a.is_contiguous() && b.is_contiguous() && like.is_contiguous()) return true;
+  return a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense() && same_strides(a, b) && same_strides(a, like);
 }
 
 bool as_list(PyObject* o) {
@@ -43,28 +49,30 @@ PyObject* guarded(F&& f) {
 
 unsigned long long* words(PyObject* o) { return static_cast<unsigned long long*>(PyLong_AsVoidPtr(o)); }
 
-// gather(params, dtype, device, sizes, param_out, grad_out) -> place of the first parameter that is not a dense tensor of that
-// element type on that device with that many elements and a gradient of the same kind and memory order; -1: all are, and the
-// addresses have been written.  sizes, param_out, grad_out: addresses of arrays as long as the list
+// gather(params, like, dtype, device, sizes, param_out, grad_out) -> place of the first parameter that is not a dense tensor of
+// that element type on that device with that many elements, the memory order of its entry of `like` (the order of its state) and
+// a gradient of the same kind and order; -1: all are, and the addresses have been written.  sizes, param_out, grad_out: addresses
+// of arrays as long as the lists
 PyObject* gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    if (nargs != 6 || !as_list(args[0])) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "gather takes six arguments");
+    if (nargs != 7 || !as_list(args[0]) || !as_list(args[1]) || PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1])) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "gather takes seven arguments, the first two of one length");
       return nullptr;
     }
-    const long dtype = PyLong_AsLong(args[1]), device = PyLong_AsLong(args[2]);
-    const unsigned long long *sizes = words(args[3]);
-    unsigned long long *pout = words(args[4]), *gout = words(args[5]);
+    const long dtype = PyLong_AsLong(args[2]), device = PyLong_AsLong(args[3]);
+    const unsigned long long *sizes = words(args[4]);
+    unsigned long long *pout = words(args[5]), *gout = words(args[6]);
     if (PyErr_Occurred()) return nullptr;
     const Py_ssize_t n = PyList_GET_SIZE(args[0]);
     for (Py_ssize_t k = 0; k < n; ++k) {
-      PyObject* o = PyList_GET_ITEM(args[0], k);
-      if (!THPVariable_Check(o)) return PyLong_FromSsize_t(k);
+      PyObject *o = PyList_GET_ITEM(args[0], k), *l = PyList_GET_ITEM(args[1], k);
+      if (!THPVariable_Check(o) || !THPVariable_Check(l)) return PyLong_FromSsize_t(k);
       const at::Tensor& p = THPVariable_Unpack(o);
       const at::Tensor& g = p.grad();
       if (!g.defined() || p.layout() != at::kStrided || g.layout() != at::kStrided || !p.is_cuda() || !g.is_cuda() ||
           p.get_device() != device || g.get_device() != device || code_of(p.scalar_type()) != dtype || code_of(g.scalar_type()) != dtype ||
-          (unsigned long long)p.numel() != sizes[k] || (unsigned long long)g.numel() != sizes[k] || !same_dense_order(p, g))
+          (unsigned long long)p.numel() != sizes[k] || (unsigned long long)g.numel() != sizes[k] || 
+          !same_dense_order(p, g, THPVariable_Unpack(l)))
         return PyLong_FromSsize_t(k);
       pout[k] = reinterpret_cast<unsigned long long>(p.data_ptr());
       gout[k] = reinterpret_cast<unsigned long long>(g.data_ptr());
@@ -111,16 +119,29 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// with_gradient(params) -> number of parameters that have one
-PyObject* with_gradient(PyObject*, PyObject* list) {
+// fits(groups, params, mask) -> whether the lists of parameters in `groups` are, one behind the other, these very objects, and
+// those with a gradient are the ones that `mask` (bytes) marks
+PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    if (!as_list(list)) return nullptr;
-    Py_ssize_t n = 0;
-    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(list); ++k) {
-      PyObject* o = PyList_GET_ITEM(list, k);
-      n += THPVariable_Check(o) && THPVariable_Unpack(o).grad().defined();
+    if (nargs != 3 || !as_list(args[0]) || !as_list(args[1]) || !PyBytes_Check(args[2]) || PyBytes_GET_SIZE(args[2]) != PyList_GET_SIZE(args[1])) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "fits takes a list of lists, a list and as many bytes");
+      return nullptr;
     }
-    return PyLong_FromSsize_t(n);
+    const char* mask = PyBytes_AS_STRING(args[2]);
+    const Py_ssize_t n = PyList_GET_SIZE(args[1]);
+    Py_ssize_t at = 0;
+    for (Py_ssize_t j = 0; j < PyList_GET_SIZE(args[0]); ++j) {
+      PyObject* group = PyList_GET_ITEM(args[0], j);
+      if (!as_list(group)) return nullptr;
+      for (Py_ssize_t k = 0; k < PyList_GET_SIZE(group); ++k, ++at) {
+        PyObject* o = PyList_GET_ITEM(group, k);
+        if (at >= n || o != PyList_GET_ITEM(args[1], at) || !THPVariable_Check(o) ||
+            THPVariable_Unpack(o).grad().defined() != (mask[at] != 0))
+          Py_RETURN_FALSE;
+      }
+    }
+    if (at != n) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
   });
 }
 
@@ -146,7 +167,7 @@ PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gradients)), METH_FASTCALL, nullptr},
-    {"with_gradient", with_gradient, METH_O, nullptr},
+    {"fits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fits)), METH_FASTCALL, nullptr},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(changed)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -412,6 +412,49 @@ def test_memory_orders(dev):
         assert float((p.grad - q.grad).abs().max()) <= 1e-6
 
 
+@pytest.mark.parametrize('dtype,master', [('float32', False), ('bfloat16', True)])
+def test_a_parameter_whose_memory_order_changes(dev, dtype, master):
+    """model.to(memory_format=channels_last) between steps: 32-bit states follow, 8-bit ones refuse"""
+    from pde_surrogate_amd import optim
+    torch.manual_seed(0)
+    ps = [torch.nn.Parameter(torch.randn(8, 6, 3, 3, device=dev, dtype=DT[dtype])), torch.nn.Parameter(torch.randn(77, device=dev, dtype=DT[dtype]))]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    a, b = (optim.FusedAdamW(x, lr=1e-2, master_weights=master) for x in (ps, qs))
+    c = optim.FusedAdamW([torch.nn.Parameter(ps[0].detach().clone())], state_bits=8)
+    for t in range(4):
+        _grads(qs, t)
+        if t == 2:
+            for x in (ps, c.param_groups[0]['params']):
+                x[0].grad = None
+                x[0].data = x[0].data.to(memory_format=torch.channels_last)
+        for p, q in zip(ps, qs):
+            p.grad = q.grad.clone(memory_format=torch.preserve_format) if t != 3 else q.grad.to(memory_format=torch.channels_last if q.dim() == 4 else torch.preserve_format)
+        a.step()
+        b.step()
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q) and float(a.state[p]['step']) == t + 1
+            assert all(torch.equal(a.state[p][k], b.state[q][k]) for k in a.state[p])
+        c.param_groups[0]['params'][0].grad = qs[0].grad.clone()
+        if t < 2:
+            c.step()
+        else:
+            with pytest.raises(RuntimeError, match='memory order'):
+                c.step()
+    assert a.state[ps[0]]['exp_avg'].stride() == ps[0].stride()
+
+
+def test_a_group_whose_parameters_are_exchanged(dev):
+    from pde_surrogate_amd import optim
+    ps = _params(dev, [10, 20])
+    _grads(ps, 0)
+    opt = optim.FusedAdamW(ps[:1], lr=1e-2)
+    opt.step()
+    keep, other = ps[0].detach().clone(), ps[1].detach().clone()
+    opt.param_groups[0]['params'][0] = ps[1]
+    opt.step()
+    assert torch.equal(ps[0], keep) and not torch.equal(ps[1], other) and float(opt.state[ps[1]]['step']) == 1
+
+
 def test_overwritten_master_weights_are_taken_as_they_are(dev):
     """the program overwrites bf16 parameters (a loaded model, a pruned weight): the kept low half moves the weight by half a
     step at most, never across zero or into infinity"""
@@ -549,7 +592,7 @@ def test_states_go_to_and_come_from_torch(dev):
         b.step()
         for p, q in zip(ps, qs):
             # each side rounds a handful of operations of an update of lr
-            assert float((p - q).abs().max()) <= 40 * au.U * (1e-3 * 10 + float(q.abs().max()))
+            assert float((p - q).detach().abs().max()) <= 40 * au.U * (1e-3 * 10 + float(q.detach().abs().max()))
             assert float(a.state[p]['step']) == float(b.state[q]['step']) == t + 1
         if t == 1:
             saved = copy.deepcopy(b.state_dict())
@@ -722,6 +765,8 @@ def test_refusals(dev):
         optim.FusedAdamW([torch.nn.Parameter(torch.zeros(4, 8, device=dev)[:, ::2])])
     with pytest.raises(ValueError, match='tensor'):
         optim.FusedAdamW([p], lr=torch.tensor(1e-3))
+    with pytest.raises(ValueError, match='float16'):
+        optim.FusedAdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float16, device=dev))], master_weights=True)
     for lr in (torch.tensor(1e-3), torch.tensor([1e-3], device=dev), torch.tensor(1e-3, device=dev, dtype=torch.float64)):
         with pytest.raises(ValueError, match='0-d float32'):
             optim.FusedAdamW([p], lr=lr, capturable=True)
