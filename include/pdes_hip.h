@@ -601,7 +601,7 @@ enum { PDES_MT_F32 = 0, PDES_MT_BF16 = 1, PDES_MT_F16 = 2 };
 int pdes_grad_norm(const unsigned long long* grads, const long long* sizes, int count, int dtype, int kind, double* rows,
                    int add, void* stream);
 /* norm_out[0] (nullable, fp32) = the norm that `rows` make, and grads *= min(1, limit / (norm + 1e-6)) in place; limit =
- * infinity finds the norm only; a factor of 1 writes nothing.  limit < 0 or NaN: PDES_EINVAL. */
+ * infinity changes nothing; a factor of 1 writes nothing.  limit < 0 or NaN: PDES_EINVAL. */
 int pdes_clip_grads(const unsigned long long* grads, const long long* sizes, int count, int dtype, int kind,
                     const double* rows, float limit, float* norm_out, void* stream);
 
@@ -625,7 +625,7 @@ typedef struct pdes_adamw_state {
   short* low;             /* bf16 parameters: the 16 bits below each (nullable: parameters are rounded to nearest) */
   long long blocks;       /* blocks that the state buffers hold */
   const double* norm_rows;/* of pdes_grad_norm: gradients are multiplied by min(1, limit / (norm + 1e-6)) as they are read */
-  float* norm_out;        /* with norm_rows: the norm is written here */
+  float* norm_out;        /* with norm_rows: the norm is written here (by a list with elements) */
   void* hyper;            /* with step_dev: PDES_MT_HYPER_BYTES of device scratch */
   float limit;
   int dtype, bits, maximize;

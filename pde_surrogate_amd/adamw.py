@@ -42,6 +42,12 @@ class AdamWState(ctypes.Structure):
 
 
 _host_module = None
+# the current stream's handle: torch.cuda.current_stream makes an object of it first, 1.8 us of the 17 that a step of one tensor takes
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def _stream(device):
+    return _raw_stream(device.index) if _raw_stream is not None else _lib.stream_ptr(device)
 
 
 def _host():
@@ -137,7 +143,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     device = torch.device('cuda', index)
     kind = 2 if norm_type == 2.0 else 0
     with _lib.device_guard(device):
-        stream = _lib.stream_ptr(device)
+        stream = _stream(device)
         rows = _norm_rows(lists, kind, device, stream)
         norm = torch.empty((), dtype=torch.float32, device=device)
 
@@ -178,7 +184,7 @@ class _Arena:
                          'rms_q': zeros(n, torch.uint8).view(torch.float8_e4m3fn), 'rms_scale': zeros(blocks, torch.float32)}
         if master and dtype == torch.bfloat16:
             self.bufs['low'] = zeros(n, torch.int16)
-        self.stream = torch.cuda.current_stream(device)
+        self.stream = _stream(device)
 
     def views(self, p, block0):
         """{name: the part of it that belongs to p}: in p's shape and order where there is one value per element"""
@@ -242,8 +248,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     place.  Without it a bf16 / fp16 parameter is rounded to nearest after every step, as torch does.
     clip_norm       gradients are multiplied by min(1, clip_norm / (norm + 1e-6)) as the step reads them, the norm taken over
                     all gradients of the step; `.grad` stays as it is, `grad_norm` is the norm (0-d tensor on the device).
-    capturable      step counts live on the device (and `lr` may be a 0-d device tensor), so that a step may be captured into
-                    a graph; take one eager step first, which makes the states.
+    capturable      step counts live on the device, so that a step may be captured into a graph; take one eager step first, which
+                    makes the states.  `lr` may be a 0-d fp32 device tensor then, read at every replay (a number is captured).
     seed            of the stochastic rounding: equal seeds, parameters and gradients give equal bits.
 
     A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
@@ -517,8 +523,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _run(self, plan, capturing):
         device, L, host = self._device, _lib.lib(), _host()
-        current = torch.cuda.current_stream(device)
-        stream = current.cuda_stream
+        stream = _stream(device)
         rows, norm = None, None
         if self.clip_norm is not None:
             lists = [(x.state.dtype, x.grad_at, x.size_at, x.count) for x in plan.launches if x.total]
@@ -557,6 +562,6 @@ class FusedAdamW(torch.optim.Optimizer):
                 for _, _, count in x.classes:
                     count += 1
             host.changed(x.params, False)
-            if x.arena.stream != current and not capturing:     # freed later than this stream's work on them
+            if x.arena.stream != stream and not capturing:      # freed later than this stream's work on them
                 for buf in x.arena.bufs.values():
-                    buf.record_stream(current)
+                    buf.record_stream(torch.cuda.current_stream(device))

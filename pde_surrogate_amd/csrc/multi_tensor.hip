@@ -203,8 +203,9 @@ __device__ __forceinline__ float whole_norm(const double* rows, double* lds) {
   return (float)(KIND == 2 ? sqrt(s) : s);
 }
 // what the gradients are multiplied by: limit / (norm + 1e-6), rounded the way torch.nn.utils.clip_grad_norm_ rounds it
-// (a reciprocal, then a product); NaN stays NaN
+// (a reciprocal, then a product); NaN stays NaN.  Without a limit nothing is changed, whatever the norm
 __device__ __forceinline__ float clip_factor(float norm, float limit) {
+  if (limit == INFINITY) return 1.f;
   const float c = 1.f / (norm + 1e-6f) * limit;
   return c > 1.f ? 1.f : c;
 }
@@ -270,7 +271,6 @@ __global__ __launch_bounds__(256) void clip_kernel(const NormArgs a) {
   __shared__ double lds[4];
   const float norm = whole_norm<KIND>(a.in, lds);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm_out) *a.norm_out = norm;
-  if (a.limit == INFINITY) return;             // the norm alone was asked for
   const float f = clip_factor(norm, a.limit);
   if (f == 1.f) return;
   const Finder<NORM_MAX> find(a.chunk0);

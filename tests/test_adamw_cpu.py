@@ -158,3 +158,29 @@ def test_cli_flags(tmp_path):
             with pytest.raises(SystemExit):
                 cli.Parser().parse(['--exp-dir', str(tmp_path / 'no')] + argv)
     assert not (tmp_path / 'no').exists()
+
+
+def test_host_functions_on_lists():
+    """_tensor_list.so on CPU tensors: patterns of gradients, version counters, and no address of anything that is not on the device"""
+    from pde_surrogate_amd.adamw import _host, _words
+    host = _host()
+    ps = [torch.nn.Parameter(torch.zeros(3)) for _ in range(4)]
+    ps[1].grad, ps[3].grad = torch.ones(3), torch.ones(3)
+    mask = bytes([0, 1, 0, 1])
+    assert host.fits([ps], ps, mask) and host.fits([ps[:1], [], ps[1:]], ps, mask)
+    assert not host.fits([ps[:3]], ps, mask) and not host.fits([ps + ps[:1]], ps, mask) and not host.fits([ps[::-1]], ps, mask)
+    assert not host.fits([ps], ps, bytes([0, 1, 1, 1])) and not host.fits([ps], ps, bytes(4))
+    before = [p._version for p in ps] + [ps[1].grad._version]
+    host.changed(ps, False)
+    assert [p._version for p in ps] == [v + 1 for v in before[:4]] and ps[1].grad._version == before[4]
+    host.changed(ps, True)
+    assert ps[1].grad._version == before[4] + 1 and [p._version for p in ps] == [v + 1 for v in before[:4]]
+    (sizes, at), (out, oat), (gout, gat) = _words(4), _words(4), _words(4)
+    assert host.gather(ps, ps, 0, 0, at, oat, gat) == 0 and not any(out)
+    assert host.gather([], [], 0, 0, at, oat, gat) == -1
+    (a, aat), (b, bat) = _words(12), _words(12)
+    assert host.gradients(ps, aat, bat)[4] == 1 and host.gradients([ps[0]], aat, bat) == (0, 0, 0, -1, -1, 0)
+    for bad in (lambda: host.gather((), ps, 0, 0, at, oat, gat), lambda: host.gather(ps, [], 0, 0, at, oat, gat), lambda: host.gather(ps),
+                lambda: host.gradients(None, aat, bat), lambda: host.fits([ps], ps, b''), lambda: host.fits(ps, ps, mask), lambda: host.changed(3, 1)):
+        with pytest.raises(TypeError):
+            bad()

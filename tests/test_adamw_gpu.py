@@ -708,6 +708,28 @@ def test_captured_steps(dev, bits, dtype, master):
         assert torch.equal(total, want) and all(torch.equal(p.grad, q.grad) for p, q in zip(ps, qs))
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_an_infinite_limit_changes_nothing(dev, bits):
+    """clip_norm = inf finds the norm of every step; a norm that is infinite or NaN leaves the other elements alone"""
+    from pde_surrogate_amd import optim
+    ps, qs = _params(dev, [300, 40]), _params(dev, [300, 40])
+    a, b = optim.FusedAdamW(ps, clip_norm=math.inf, state_bits=bits), optim.FusedAdamW(qs, state_bits=bits)
+    for x in (1.0, math.inf, math.nan):
+        _grads(ps, 1)
+        ps[0].grad[5] = x
+        for p, q in zip(ps, qs):
+            q.grad = p.grad.clone()
+        a.step()
+        b.step()
+        norm = float(a.grad_norm)
+        assert math.isnan(norm) if math.isnan(x) else norm == math.inf if math.isinf(x) else norm > 1
+        for p, q in zip(ps, qs):
+            assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p[~p.isnan()], q[~q.isnan()])
+    a.clip_norm = None
+    a.step()
+    assert a.grad_norm is None
+
+
 def test_autograd_sees_the_step(dev):
     """a parameter changed between a forward and its backward is caught, as with any in-place change"""
     from pde_surrogate_amd import optim
