@@ -10,6 +10,12 @@ import torch
 import adamw_util as au
 
 
+@pytest.fixture(scope='module', autouse=True)
+def _built():
+    from pde_surrogate_amd import build
+    build.build(verbose=False)                 # (nothing to do where everything is built)
+
+
 def test_arguments_are_checked_before_anything_else():
     from pde_surrogate_amd import optim
     p = [torch.nn.Parameter(torch.zeros(3))]

@@ -536,6 +536,28 @@ def test_gradients_that_come_and_go_and_many_groups(dev, bits):
             assert float((p - q).detach().float().abs().max()) <= 5e-3 * (k + 1) * 5
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_thousand_tensors(dev, bits):
+    """eleven launches and seven for the norm: all of them step by the one norm, as the same numbers do in one tensor"""
+    from pde_surrogate_amd import optim
+    flat = torch.randn(1000 * 256, device=dev)
+    g = torch.randn_like(flat)
+    ps = [torch.nn.Parameter(x.clone()) for x in flat.split(256)]
+    one = torch.nn.Parameter(flat.clone())
+    one.grad = g.clone()
+    for p, x in zip(ps, g.split(256)):
+        p.grad = x.clone()
+    a, b = optim.FusedAdamW(ps, clip_norm=3.0, state_bits=bits), optim.FusedAdamW([one], clip_norm=3.0, state_bits=bits)
+    for _ in range(2):
+        a.step()
+        b.step()
+        assert torch.equal(a.grad_norm, b.grad_norm)
+        if bits == 32 or _ == 0:               # (8-bit codes are rounded by the tensors' places)
+            assert torch.equal(torch.cat([p.detach() for p in ps]), one.detach())
+    n = optim.clip_grad_norm_(ps, 1.0)
+    assert torch.equal(n, optim.clip_grad_norm_(one, 1.0)) and torch.equal(torch.cat([p.grad for p in ps]), one.grad)
+
+
 def test_no_gradients_at_all_and_empty_tensors(dev):
     from pde_surrogate_amd import optim
     ps = _params(dev, [0, 0])
