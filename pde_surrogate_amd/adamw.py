@@ -79,6 +79,11 @@ def _same_order(a, b):
     return all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
 
 
+def _order(t):
+    """the dimensions of a dense tensor from the outermost in memory to the innermost; those of one element have no place"""
+    return tuple(sorted((d for d in range(t.dim()) if t.shape[d] != 1), key=lambda d: -t.stride(d)))
+
+
 def _check_tensor(t, what):
     if t.layout != torch.strided:
         raise RuntimeError(f'{what}: sparse tensors are not supported')
@@ -382,6 +387,10 @@ class FusedAdamW(torch.optim.Optimizer):
         sd = super().state_dict()
         # here parameters that are stepped together share one count; another optimiser would count it once for each of them
         sd['state'] = {k: {**v, 'step': v['step'].clone()} if 'step' in v else v for k, v in sd['state'].items()}
+        if self.state_bits == 8:           # whose blocks belong to stretches of memory, whatever the shape
+            for k, p in enumerate(p for g in self.param_groups for p in g['params']):
+                if 'step' in sd['state'].get(k, ()):
+                    sd['state'][k]['order'] = _order(self._where[p][2] if p in self._where else p)
         return sd
 
     @torch.no_grad()
@@ -396,6 +405,9 @@ class FusedAdamW(torch.optim.Optimizer):
             # the base class would convert the states to their parameters' type: it gets the groups alone
             super().load_state_dict({'state': {}, 'param_groups': groups})
             self.state = defaultdict(dict, {p: dict(saved[i]) for i, p in zip(theirs, ours) if saved.get(i)})
+            for p, st in self.state.items():
+                if tuple(st.pop('order', _order(p))) != _order(p):
+                    raise ValueError('load_state_dict: the 8-bit state of a parameter belongs to another memory order than it has')
             for g in self.param_groups:
                 self._check_group(g)
             with _lib.device_guard(self._device):

@@ -49,12 +49,14 @@ def test_torch_optimisers_are_still_the_modules_own():
 
 
 def test_memory_order_helpers():
-    from pde_surrogate_amd.adamw import _dense, _overlap, _same_order
+    from pde_surrogate_amd.adamw import _dense, _order, _overlap, _same_order
     x = torch.zeros(4, 6, 2)
     assert _dense(x) and _dense(x.permute(2, 0, 1)) and _dense(x[1]) and _dense(torch.zeros(())) and _dense(torch.zeros(0, 3))
     assert not _dense(x[:, ::2]) and not _dense(x[:, :3]) and not _dense(torch.zeros(1, 1).expand(3, 3)) and not _dense(x.as_strided((3, 3), (1, 1)))
     assert _same_order(x, torch.ones(4, 6, 2)) and not _same_order(x, torch.ones(6, 4, 2).permute(1, 0, 2))
     assert _same_order(torch.zeros(1, 5), torch.zeros(5, 1).t())
+    assert _order(x) == (0, 1, 2) and _order(x.permute(2, 0, 1)) == (1, 2, 0) and _order(torch.zeros(())) == ()
+    assert _order(torch.zeros(1, 5)) == _order(torch.zeros(5, 1).t()) == (1,)
     assert _overlap([(8, 4), (8, 8)]) and _overlap([(20, 8), (8, 13)]) and not _overlap([(20, 8), (8, 12), (0, 0), (0, 0), (10, 0)])
 
 

@@ -601,6 +601,25 @@ def test_saved_and_copied_states_go_on_bit_for_bit(dev, tmp_path, bits, dtype, m
                 assert torch.equal(a.state[p][k].reshape(-1).view(torch.uint8), o.state[q][k].reshape(-1).view(torch.uint8)), k
 
 
+def test_saved_8_bit_states_load_into_their_own_memory_order_only(dev):
+    from pde_surrogate_amd import optim
+    x = torch.randn(8, 5, 3, 3, device=dev)
+    a, b, c = (torch.nn.Parameter(y) for y in (x.to(memory_format=torch.channels_last), x.clone(), x.to(memory_format=torch.channels_last)))
+    opts = [optim.FusedAdamW([p], state_bits=8) for p in (a, b, c)]
+    for p, o in zip((a, b, c), opts):
+        p.grad = torch.ones_like(p)
+        o.step()
+    sd = opts[0].state_dict()
+    held, codes = b.detach().clone(), opts[1].state[b]['rms_q'].view(torch.uint8).clone()
+    with pytest.raises(ValueError, match='memory order'):
+        opts[1].load_state_dict(sd)
+    assert torch.equal(opts[1].state[b]['rms_q'].view(torch.uint8), codes) and torch.equal(b, held)
+    opts[2].load_state_dict(sd)
+    for o, p in ((opts[0], a), (opts[2], c)):
+        o.step()
+    assert torch.equal(a, c) and 'order' not in opts[2].state[c]
+
+
 def test_states_go_to_and_come_from_torch(dev):
     from pde_surrogate_amd import optim
     ps = _params(dev, [50, 3000])
