@@ -469,7 +469,7 @@ constexpr int ODD_ROOT = 0x290;              // class mask: subnormal numbers an
 
 // A half wave holds a block, a lane eight elements of it: consecutive ones of 16 bits, or twice four of 32 bits, 128 elements
 // apart, so that each access of a wave covers whole lines (332 M fp32 parameters, streaming: 852 us; eight consecutive ones, two
-// accesses to each half of a line: 975 us). 
+// accesses to each half of a line: 975 us).
 template <class T>
 struct Share {
   static constexpr int PER = sizeof(typename T::E) == 4 ? 4 : 8, PARTS = 8 / PER, APART = 128;
@@ -769,7 +769,7 @@ extern "C" int pdes_grad_norm(const unsigned long long* grads, const long long* 
   a.out = rows; a.norm_out = nullptr; a.limit = 0.f;
   long long total = 0;
   for (int k = 0; k < count; ++k) total += sizes[k] > 0 && sizes[k] < MT_LONGEST ? sizes[k] : 0;
-  const long long bytes = total * item_size(dtype), 
+  const long long bytes = total * item_size(dtype),
                   chunk = (bytes > SHORT_MOST ? LONG_THREADS : SHORT_THREADS) * NORM_U * 16ll / item_size(dtype);
   int done = 0;
   do {                            // (an empty list still writes its rows)
@@ -829,7 +829,7 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
   for (int k = 0; k < count; ++k) {
     const pdes_mt_tensor& t = tensors[k];
     if (t.n < 0 || t.n >= MT_LONGEST - total || t.block0 < 0 || t.cls < 0 || t.cls >= nclasses) return PDES_EINVAL;
-    if (t.block0 + (t.n + MT_BLOCK - 1) / MT_BLOCK > s.blocks) return PDES_EINVAL;
+    if (t.block0 > s.blocks || t.block0 + (t.n + MT_BLOCK - 1) / MT_BLOCK > s.blocks) return PDES_EINVAL;
     if (t.n && (!params[k] || !grads[k])) return PDES_EINVAL;
     if (params[k] % size || grads[k] % size) return PDES_EALIGN;
     total += t.n;

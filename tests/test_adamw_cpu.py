@@ -91,7 +91,7 @@ def test_c_entries_refuse_what_the_kernels_do_not_take():
                                  (AdamWClass * 1)(AdamWClass(*cls)), nclasses, ctypes.byref(st), None)
     for kw in (dict(count=-1), dict(nclasses=0), dict(nclasses=9), dict(bits=16), dict(dtype=3), dict(low=4096), dict(blocks=0), dict(blocks=-1),
                dict(params=0), dict(grads=0), dict(exp_avg=None), dict(exp_avg_sq=None), dict(bits=8, rms_scale=None),
-               dict(tensor=(257, 0, 0, 0)), dict(tensor=(10, 1, 0, 0)), dict(tensor=(10, -1, 0, 0)), dict(tensor=(-1, 0, 0, 0)),
+               dict(tensor=(257, 0, 0, 0)), dict(tensor=(10, 1, 0, 0)), dict(tensor=(10, -1, 0, 0)), dict(tensor=(10, (1 << 63) - 1, 0, 0)), dict(tensor=(-1, 0, 0, 0)),
                dict(tensor=(10, 0, 1, 0)), dict(tensor=(10, 0, -1, 0)), dict(norm_rows=4096, limit=-1.0), dict(norm_rows=4096, limit=math.nan),
                dict(cls=(1e-3, 1.0, 0.99, 1e-8, 0.0, 1, None, None)), dict(cls=(1e-3, 0.9, math.nan, 1e-8, 0.0, 1, None, None)),
                dict(cls=(1e-3, 0.9, 0.99, -1.0, 0.0, 1, None, None)), dict(cls=(1e-3, 0.9, 0.99, 1e-8, 0.0, 0, None, None)),
