@@ -398,6 +398,8 @@ class FusedAdamW(torch.optim.Optimizer):
         saved, groups = state_dict['state'], state_dict['param_groups']
         if any(g.get('amsgrad') for g in groups):
             raise ValueError('load_state_dict: amsgrad states are not supported')
+        if any(bool(g.get('maximize', self.maximize)) != self.maximize for g in groups):
+            raise ValueError(f'load_state_dict: maximize is {not self.maximize} in the dictionary and {self.maximize} here (a choice of the constructor)')
         ours, theirs = [p for g in self.param_groups for p in g['params']], [i for g in groups for i in g['params']]
         before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_retired', '_where', '_arenas', '_plan')}
         steps = [st['step'] for st in self.state.values() if 'step' in st]

@@ -601,6 +601,20 @@ def test_saved_and_copied_states_go_on_bit_for_bit(dev, tmp_path, bits, dtype, m
                 assert torch.equal(a.state[p][k].reshape(-1).view(torch.uint8), o.state[q][k].reshape(-1).view(torch.uint8)), k
 
 
+@pytest.mark.parametrize('ours', [False, True])
+def test_states_of_an_optimiser_that_goes_the_other_way_are_refused(dev, ours):
+    from pde_surrogate_amd import optim
+    p, q = (torch.nn.Parameter(torch.ones(5, device=dev)) for _ in range(2))
+    opt = optim.FusedAdamW([p], maximize=ours)
+    with pytest.raises(ValueError, match='maximize'):
+        opt.load_state_dict(torch.optim.AdamW([q], maximize=not ours).state_dict())
+    opt.load_state_dict(torch.optim.AdamW([q], maximize=ours).state_dict())
+    opt.load_state_dict(optim.FusedAdamW([q], maximize=ours).state_dict())
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert ((p > 1) if ours else (p < 1)).all()
+
+
 def test_saved_8_bit_states_load_into_their_own_memory_order_only(dev):
     from pde_surrogate_amd import optim
     x = torch.randn(8, 5, 3, 3, device=dev)
