@@ -91,6 +91,9 @@ extern "C" int pdes_context_device(const pdes_context* ctx) {
   return ctx ? reinterpret_cast<const Context*>(ctx)->device : PDES_EINVAL;
 }
 
+// the version of include/pdes_hip.h (here, where no measured kernel's source changes with it)
+extern "C" int pdes_abi_version(void) { return 25; }
+
 // sizeof of the structures that cross the boundary (the ctypes mirrors are checked against it: tests/test_cabi.py)
 extern "C" int pdes_sizeof(int which) {
   switch (which) {

@@ -596,5 +596,3 @@ extern "C" int pdes_sobel5_grad_adjoint(const float* gh_bar, const float* gv_bar
   PDES_LAUNCH_CHECK();
   return PDES_OK;
 }
-
-extern "C" int pdes_abi_version(void) { return 25; }
