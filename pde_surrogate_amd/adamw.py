@@ -13,6 +13,7 @@ import ctypes
 import math
 from array import array
 from collections import defaultdict
+from operator import is_
 
 import torch
 
@@ -235,11 +236,13 @@ class _Reordered(Exception):
 
 
 class _Plan:
-    """the launches of a step, for as long as the same parameters have gradients and the states are the same"""
+    """the launches of a step, for as long as the same parameters of the same groups have gradients and the states are the same"""
 
-    def __init__(self, launches, params, state):
-        self.launches, self.params, self.state, self.states = launches, params, state, len(state)
-        self.mask = bytes(p.grad is not None for p in params)
+    def __init__(self, launches, groups, state):
+        self.launches, self.state, self.states = launches, state, len(state)
+        self.groups, self.counts = list(groups), [len(g['params']) for g in groups]
+        self.params = [p for g in groups for p in g['params']]
+        self.mask = bytes(p.grad is not None for p in self.params)
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -467,7 +470,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 part = keys[at:at + _CLASSES]
                 members = sorted(((p, c, b, o, like) for c, key in enumerate(part) for p, b, o, like in classes[key][3]), key=lambda m: m[3])
                 launches.append(_Launch(arena, members, [(classes[key][1], counted[key]) for key in part]))
-        self._plan = _Plan(launches, [p for _, p in every], self.state)
+        self._plan = _Plan(launches, self.param_groups, self.state)
         return self._plan
 
     @torch.no_grad()
@@ -532,8 +535,11 @@ class FusedAdamW(torch.optim.Optimizer):
             self._retire(self._where.pop(p), self.state[p])
 
     def _fits(self, plan):
+        groups, lists = self.param_groups, [g['params'] for g in self.param_groups]
         return (plan.state is self.state and plan.states == len(self.state) and
-                _host().fits([g['params'] for g in self.param_groups], plan.params, plan.mask))
+                # the plan's constants come from these dictionaries, whose parameters stand one behind the other in plan.params
+                len(groups) == len(plan.groups) and all(map(is_, groups, plan.groups)) and [len(x) for x in lists] == plan.counts and
+                _host().fits(lists, plan.params, plan.mask))
 
     def _run(self, plan, capturing):
         device, L, host = self._device, _lib.lib(), _host()
