@@ -190,6 +190,7 @@ class _Arena:
                          'rms_q': zeros(n, torch.uint8).view(torch.float8_e4m3fn), 'rms_scale': zeros(blocks, torch.float32)}
         if master and dtype == torch.bfloat16:
             self.bufs['low'] = zeros(n, torch.int16)
+        self.names = {'step', *self.bufs}
         self.stream = _stream(device)
 
     def views(self, p, block0):
@@ -236,10 +237,10 @@ class _Reordered(Exception):
 
 
 class _Plan:
-    """the launches of a step, for as long as the same parameters of the same groups have gradients and the states are the same"""
+    """the launches of a step, for as long as the same parameters of the same groups have gradients and no state is replaced"""
 
-    def __init__(self, launches, groups, state):
-        self.launches, self.state, self.states = launches, state, len(state)
+    def __init__(self, launches, groups):
+        self.launches = launches
         self.groups, self.counts = list(groups), [len(g['params']) for g in groups]
         self.params = [p for g in groups for p in g['params']]
         self.mask = bytes(p.grad is not None for p in self.params)
@@ -259,6 +260,9 @@ class FusedAdamW(torch.optim.Optimizer):
     capturable      step counts live on the device, so that a step may be captured into a graph; take one eager step first, which
                     makes the states.  `lr` may be a 0-d fp32 device tensor then, read at every replay (a number is captured).
     seed            of the stochastic rounding: equal seeds, parameters and gradients give equal bits.
+
+    `state` may be changed as torch.optim.AdamW's may: entries replaced, a state emptied or put back.  Parameters of a group that have
+    taken equally many steps share one 'step' tensor, which an in-place change alters for all of them.
 
     A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
     dense, and no two may share memory.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse
@@ -286,9 +290,11 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     def _reset(self):
-        self._where = {}            # parameter -> (arena, block0, a tensor without memory of the parameter's shape and order then)
+        # parameter -> (arena, block0, a tensor without memory of the parameter's shape and order then, its state's tensors there)
+        self._where = {}
         self._arenas = []
         self._plan = None
+        self._known = None          # the states as the last plan found or made them (see _holds)
 
     def _retire(self, *what):
         """a captured graph may still write to buffers that have been replaced: they stay until the optimiser goes"""
@@ -337,16 +343,17 @@ class FusedAdamW(torch.optim.Optimizer):
 
     # -- states ----------------------------------------------------------------------------------------------------------
     def _make_states(self, params):
-        """states of parameters that have none, or have some from elsewhere (a loaded or copied state): one arena per type"""
-        by_type, steps, to, source = {}, {}, [], []
+        """states of parameters that have none, or have some from elsewhere (a loaded, copied or replaced state): one arena per
+        type.  Nothing is changed unless all of them fit"""
+        by_type, steps, to, source, made, arenas = {}, {}, [], [], [], []
         for p in params:
             by_type.setdefault(p.dtype, []).append(p)
         for dtype, ps in by_type.items():
             arena = _Arena(dtype, sum(-(-p.numel() // BLOCK) for p in ps), self.state_bits, self.master_weights, self._device)
-            self._arenas.append(arena)
+            arenas.append(arena)
             block0 = 0
             for p in ps:
-                mine, had = arena.views(p, block0), self.state[p]
+                mine, had = arena.views(p, block0), self.state.get(p)
                 if had:
                     for name, view in mine.items():
                         if name not in had:
@@ -357,15 +364,56 @@ class FusedAdamW(torch.optim.Optimizer):
                             raise ValueError(f'state {name!r} has shape {tuple(old.shape)}, the parameter needs {tuple(view.shape)}')
                         to.append(view)
                         source.append(old)
+                    if 'step' not in had:
+                        raise ValueError("the state of a parameter has no 'step'")
                 count = float(had['step']) if had else 0.0
                 if count not in steps:
                     steps[count] = torch.tensor(count, dtype=torch.float32, device=self._device if self.capturable else 'cpu')
-                self.state[p] = {'step': steps[count], **mine}
-                self._where[p] = (arena, block0, torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device='meta'))
+                made.append((p, {'step': steps[count], **mine}, (arena, block0, torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device='meta'),
+                                                                 [(name, view, view.data_ptr()) for name, view in mine.items()])))
                 block0 += -(-p.numel() // BLOCK)
         if to:
             with torch.no_grad():
                 torch._foreach_copy_(to, source)
+        self._arenas += arenas
+        for p, state, where in made:
+            self.state[p], self._where[p] = state, where
+
+    # A program may replace what `state` holds: an entry, the state of a parameter, all of it.  The kernels work on the arenas, so
+    # each step compares, and what is not the arena's any more is copied into a new one, as a loaded state is
+    def _know(self):
+        """notes the states as they are"""
+        known, dicts, tensors = [], [], {}
+        for p, state in self.state.items():
+            where = self._where.get(p)
+            if where is None:
+                continue
+            names = where[0].names
+            known += (p, state)
+            dicts.append(state)
+            for item in state.items():
+                if item[0] in names:
+                    known += item
+                    tensors[id(item[1])] = item[1]
+            known.append(None)
+        tensors = list(tensors.values())
+        note, at = _words(1 + len(dicts) + 2 * len(tensors))
+        _host().note(self.state, dicts, tensors, at)
+        self._known = (known, dicts, tensors, at), note
+
+    def _holds(self):
+        return self._known is not None and _host().held(self.state, *self._known[0])
+
+    def _sift(self):
+        """parameters whose states are no longer where they were made lose their place"""
+        self._plan = self._known = None
+        for p, (_, _, _, views) in list(self._where.items()):
+            st = self.state.get(p)
+            if not (st and 'step' in st and all(st.get(name) is view and view.data_ptr() == at for name, view, at in views)):
+                del self._where[p]
+        used = {id(where[0]) for where in self._where.values()}
+        self._retire([a for a in self._arenas if id(a) not in used])
+        self._arenas = [a for a in self._arenas if id(a) in used]
 
     def flat_state(self):
         """{name: [the flat buffers that hold this state, one per element type]}: the parameters' states one behind the other
@@ -431,46 +479,55 @@ class FusedAdamW(torch.optim.Optimizer):
         if capturing:
             raise RuntimeError('FusedAdamW: the first step, and the first one with gradients for other parameters than before, cannot '
                                'be captured into a graph: take it eagerly')
-        if self._where and not any('step' in self.state.get(p, ()) for p in self._where):
-            self._retire(self._arenas)
-            self._reset()                  # the program has emptied the states, or put others in their place
+        same = self._holds()
+        if not same:
+            self._sift()
         if _overlap([(p.data_ptr(), p.numel() * p.element_size()) for _, p, _ in active]):
             raise RuntimeError('FusedAdamW: two parameters share their memory')
-        new = [p for _, p, _ in active if p not in self._where or 'step' not in self.state.get(p, ())]
+        new = [p for _, p, _ in active if p not in self._where]
         if new:
             self._make_states(new)
         # a class: a group's parameters of one arena at the same step.  They share one count, which the call increments once.
         # On the device the values are unknown: there, what has shared a count so far goes on sharing it
-        holders, classes, values = {}, {}, {}
-        if self.capturable:
+        holders, classes, values, counts = {}, {}, {}, {}
+        count_device = self._device if self.capturable else torch.device('cpu')
+        if self.capturable and same:
             for p in self._where:
-                step = self.state.get(p, {}).get('step')
+                step = self.state[p]['step']
                 holders[id(step)] = holders.get(id(step), 0) + 1
         for g, p, k in active:
-            (arena, block0, like), step = self._where[p], self.state[p]['step']
+            (arena, block0, like, _), st = self._where[p], self.state[p]
+            step = st['step']
             value = values.get(id(step))
+            if value is None and not (isinstance(step, torch.Tensor) and step.dim() == 0 and step.dtype == torch.float32 and step.device == count_device):
+                count = float(step)                # (put there by the program)
+                if count not in counts:
+                    counts[count] = torch.tensor(count, dtype=torch.float32, device=count_device)
+                step = counts[count]
+                value = values.get(id(step))
             if value is None:
                 value = values[id(step)] = id(step) if self.capturable else float(step)
             key = (id(arena), id(g), value)
             if key not in classes:
                 classes[key] = (arena, g, step, [])
-            classes[key][3].append((p, block0, k, like))
+            classes[key][3].append((p, block0, k, like, st))
         counted = {}
         for key, (arena, g, step, members) in classes.items():
-            if not (self.capturable and holders[id(step)] == len(members)):
+            if holders.get(id(step)) != len(members):      # (the program may hold the count of a state that it has replaced)
                 self._retire(step)
                 step = step.clone()
-            for p, _, _, _ in members:
-                self.state[p]['step'] = step
+            for _, _, _, _, st in members:
+                st['step'] = step
             counted[key] = step
         launches = []
         for arena in self._arenas:
             keys = [k for k in classes if k[0] == id(arena)]
             for at in range(0, len(keys), _CLASSES):
                 part = keys[at:at + _CLASSES]
-                members = sorted(((p, c, b, o, like) for c, key in enumerate(part) for p, b, o, like in classes[key][3]), key=lambda m: m[3])
+                members = sorted(((p, c, b, o, like) for c, key in enumerate(part) for p, b, o, like, _ in classes[key][3]), key=lambda m: m[3])
                 launches.append(_Launch(arena, members, [(classes[key][1], counted[key]) for key in part]))
-        self._plan = _Plan(launches, self.param_groups, self.state)
+        self._plan = _Plan(launches, self.param_groups)
+        self._know()
         return self._plan
 
     @torch.no_grad()
@@ -531,12 +588,12 @@ class FusedAdamW(torch.optim.Optimizer):
         """states of parameters whose memory has got another order: 32-bit ones move into it, 8-bit ones (blocks of memory) cannot"""
         if self.state_bits == 8:
             raise RuntimeError('FusedAdamW: a parameter has another memory order than its 8-bit state')
-        for p in [p for p, (_, _, like) in self._where.items() if not _same_order(p, like)]:
+        for p in [p for p, (_, _, like, _) in self._where.items() if not _same_order(p, like)]:
             self._retire(self._where.pop(p), self.state[p])
 
     def _fits(self, plan):
         groups, lists = self.param_groups, [g['params'] for g in self.param_groups]
-        return (plan.state is self.state and plan.states == len(self.state) and
+        return (self._holds() and
                 # the plan's constants come from these dictionaries, whose parameters stand one behind the other in plan.params
                 len(groups) == len(plan.groups) and all(map(is_, groups, plan.groups)) and [len(x) for x in lists] == plan.counts and
                 _host().fits(lists, plan.params, plan.mask))

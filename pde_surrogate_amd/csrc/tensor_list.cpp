@@ -145,6 +145,110 @@ PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// ---- the states of an optimiser, compared with what they were
+// `known`: for each parameter the parameter, the dictionary of its state, pairs of a name and a tensor, and None, in the order of
+// the dictionaries; `dicts`: those dictionaries; `tensors`: those tensors, each once.  A note is an array of 1 + len(dicts) + 2
+// len(tensors) numbers: the version of `state`, of each dictionary, and where each tensor's memory is
+
+// changes with every change of a dictionary and is never the same for two (0: this Python has none, and every dictionary is read)
+uint64_t version_of(PyObject* dict) {
+#if PY_VERSION_HEX < 0x030C0000
+  return reinterpret_cast<PyDictObject*>(dict)->ma_version_tag;
+#else
+  return 0;
+#endif
+}
+// a tensor's storage, which views of one buffer share, and its place there
+bool place_of(PyObject* o, unsigned long long (&at)[2]) {
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.layout() != at::kStrided || !t.has_storage()) return false;
+  at[0] = reinterpret_cast<unsigned long long>(t.unsafeGetTensorImpl()->unsafe_storage().unsafeGetStorageImpl());
+  at[1] = static_cast<unsigned long long>(t.storage_offset());
+  return true;
+}
+void note_versions(PyObject* state, PyObject* dicts, unsigned long long* note) {
+  *note++ = version_of(state);
+  for (Py_ssize_t k = 0; k < PyList_GET_SIZE(dicts); ++k) *note++ = version_of(PyList_GET_ITEM(dicts, k));
+}
+// whether the dictionaries hold what `known` lists; what else they hold is the program's own
+bool as_known(PyObject* dict, PyObject* known) {
+  const Py_ssize_t n = PyList_GET_SIZE(known);
+  Py_ssize_t k = 0, i = 0;
+  PyObject *p, *state, *name, *value;
+  while (k < n && PyDict_Next(dict, &i, &p, &state)) {
+    if (p != PyList_GET_ITEM(known, k)) continue;
+    if (++k >= n || state != PyList_GET_ITEM(known, k)) return false;
+    ++k;
+    Py_ssize_t j = 0;
+    while (k + 1 < n && PyList_GET_ITEM(known, k) != Py_None && PyDict_Next(state, &j, &name, &value)) {
+      if (name != PyList_GET_ITEM(known, k)) continue;
+      if (value != PyList_GET_ITEM(known, k + 1)) return false;
+      k += 2;
+    }
+    if (k >= n || PyList_GET_ITEM(known, k) != Py_None) return false;
+    ++k;
+  }
+  return k == n;
+}
+bool all_dicts(PyObject* list) {
+  for (Py_ssize_t k = 0; k < PyList_GET_SIZE(list); ++k)
+    if (!PyDict_Check(PyList_GET_ITEM(list, k))) return false;
+  return true;
+}
+
+// note(state, dicts, tensors, out)
+PyObject* note(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 4 || !PyDict_Check(args[0]) || !as_list(args[1]) || !as_list(args[2]) || !all_dicts(args[1])) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "note takes a dictionary, a list of them, a list of tensors and an address");
+      return nullptr;
+    }
+    unsigned long long *out = words(args[3]), place[2];
+    if (PyErr_Occurred()) return nullptr;
+    note_versions(args[0], args[1], out);
+    out += 1 + PyList_GET_SIZE(args[1]);
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(args[2]); ++k) {
+      if (!place_of(PyList_GET_ITEM(args[2], k), place)) {
+        PyErr_SetString(PyExc_TypeError, "note takes tensors with a storage");
+        return nullptr;
+      }
+      *out++ = place[0];
+      *out++ = place[1];
+    }
+    Py_RETURN_NONE;
+  });
+}
+
+// held(state, known, dicts, tensors, note) -> whether nothing of it has been replaced since the note was made
+PyObject* held(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 5 || !PyDict_Check(args[0]) || !as_list(args[1]) || !as_list(args[2]) || !as_list(args[3])) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "held takes a dictionary, three lists and an address");
+      return nullptr;
+    }
+    unsigned long long *noted = words(args[4]), place[2];
+    if (PyErr_Occurred()) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(args[2]);
+    bool same = noted[0] != 0 && version_of(args[0]) == noted[0];
+    for (Py_ssize_t k = 0; same && k < n; ++k) same = version_of(PyList_GET_ITEM(args[2], k)) == noted[1 + k];
+    if (!same) {
+      if (!as_known(args[0], args[1])) Py_RETURN_FALSE;
+      note_versions(args[0], args[2], noted);
+    }
+    const unsigned long long* at = noted + 1 + n;
+    // (the objects are all over the heap: 2,000 of them between other work take 15 us less when the next ones are on their way)
+    const Py_ssize_t m = PyList_GET_SIZE(args[3]), ahead = 8;
+    for (Py_ssize_t k = 0; k < m; ++k, at += 2) {
+      if (k + 2 * ahead < m) __builtin_prefetch(PyList_GET_ITEM(args[3], k + 2 * ahead));
+      if (k + ahead < m && THPVariable_Check(PyList_GET_ITEM(args[3], k + ahead)))
+        __builtin_prefetch(THPVariable_Unpack(PyList_GET_ITEM(args[3], k + ahead)).unsafeGetTensorImpl());
+      if (!place_of(PyList_GET_ITEM(args[3], k), place) || place[0] != at[0] || place[1] != at[1]) Py_RETURN_FALSE;
+    }
+    Py_RETURN_TRUE;
+  });
+}
+
 // changed(params, gradients): autograd's version counters move, as after any in-place change, of the tensors or their gradients
 PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
@@ -168,6 +272,8 @@ PyMethodDef methods[] = {
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gradients)), METH_FASTCALL, nullptr},
     {"fits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fits)), METH_FASTCALL, nullptr},
+    {"note", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(note)), METH_FASTCALL, nullptr},
+    {"held", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(held)), METH_FASTCALL, nullptr},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(changed)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

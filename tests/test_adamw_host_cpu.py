@@ -85,3 +85,198 @@ def test_a_group_that_another_dictionary_replaces(entries):
     for _, opt in x.both():
         opt.param_groups = [dict(g, lr=g['lr'] * 2) for g in opt.param_groups]
     x.step()
+
+
+# ---- states that the program replaces -------------------------------------------------------------------------------------
+def _entry(name, make):
+    def change(opt, p):
+        opt.state[p][name] = make(opt.state[p][name])
+    return change
+
+
+def _emptied(opt, p):
+    opt.state[p] = {}
+
+
+def _cleared(opt, p):
+    opt.state[p].clear()
+
+
+def _deleted(opt, p):
+    del opt.state[p]
+
+
+def _other_memory(opt, p):
+    opt.state[p]['exp_avg'].data = opt.state[p]['exp_avg'].data * 0.5
+
+
+def _copied(opt, p):
+    opt.state[p] = {k: v.clone() for k, v in opt.state[p].items()}
+    opt.state[p]['exp_avg_sq'].mul_(9)
+
+
+def _all_copied(opt, p):
+    opt.state = type(opt.state)(dict, {k: {n: x.clone() for n, x in v.items()} for k, v in opt.state.items()})
+    opt.state[p]['exp_avg'].mul_(-1)
+
+
+CHANGES = {'exp_avg': _entry('exp_avg', torch.zeros_like), 'exp_avg_sq': _entry('exp_avg_sq', lambda x: x * 4), 'step': _entry('step', lambda x: torch.tensor(0.0)),
+           'step further': _entry('step', lambda x: torch.tensor(1000.0)), 'same step': _entry('step', lambda x: x.clone()),
+           'emptied': _emptied, 'cleared': _cleared, 'deleted': _deleted, 'other memory': _other_memory, 'copied': _copied, 'all copied': _all_copied}
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+@pytest.mark.parametrize('change', sorted(CHANGES))
+def test_replaced_states_are_taken(entries, change, capturable):
+    x = Pair([5, 300, 7, 256], groups=2)
+    if capturable:
+        from pde_surrogate_amd import optim
+        x.ours = optim.FusedAdamW(x.ours.param_groups, capturable=True)
+    for _ in range(2):
+        x.step()
+    for k in (1, 2, 1):
+        for ps, opt in x.both():
+            CHANGES[change](opt, ps[k])
+        x.step()
+        x.step()
+    x.step(which=(0, 3))
+    x.step()
+    for ps, opt in x.both():                       # while the parameter has no gradient
+        CHANGES[change](opt, ps[3])
+    x.step(which=(0, 1))
+    x.step()
+    a, b = x.ours.state_dict()['state'], x.torch.state_dict()['state']
+    assert all(torch.allclose(a[k][n], b[k][n], rtol=1e-4, atol=1e-5) for k in b for n in b[k])
+
+
+def test_a_count_that_is_a_number(entries):
+    x = Pair([5, 300, 7], groups=1)
+    x.step()
+    for k in (0, 1, 2):
+        x.ours.state[x.ps[k]]['step'] = 7
+        x.torch.state[x.qs[k]]['step'] = torch.tensor(7.0)
+    x.step()
+    x.ours.state[x.ps[1]]['step'] = torch.tensor(3, dtype=torch.int64)
+    x.torch.state[x.qs[1]]['step'] = torch.tensor(3.0)
+    x.step()
+    assert entries.launches == [3] * 3
+
+
+def test_a_shared_count_that_changes_in_place_or_moves(entries):
+    """parameters that are stepped together share one count here; in torch's optimiser each has its own"""
+    x = Pair([5, 300, 7], groups=1)
+    x.step()
+    for move in (False, True):
+        for ps, opt in x.both():
+            for p in ps:
+                if move:
+                    opt.state[p]['step'].data = torch.tensor(40.0)
+                else:
+                    opt.state[p]['step'].fill_(11)
+                if opt is x.ours:
+                    break
+        x.step()
+    assert entries.launches == [3] * 3
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+def test_states_that_are_taken_out_and_put_back(entries, capturable):
+    """the tensors that a program holds are its own: nothing writes to them once others have taken their place"""
+    x = Pair([5, 300, 7])
+    if capturable:
+        from pde_surrogate_amd import optim
+        x.ours = optim.FusedAdamW(x.ours.param_groups, capturable=True)
+    x.step()
+    x.step()
+    held = [opt.state[ps[1]] for ps, opt in x.both()]
+    moment = [opt.state[ps[2]]['exp_avg'] for ps, opt in x.both()]
+    copies = {k: v.clone() for k, v in held[0].items()}, moment[0].clone()
+    for ps, opt in x.both():
+        opt.state[ps[1]] = {}
+        opt.state[ps[2]]['exp_avg'] = torch.ones(7)
+    x.step()
+    x.step()
+    assert all(torch.equal(held[0][k], v) for k, v in copies[0].items() if k != 'step') and torch.equal(moment[0], copies[1])
+    assert float(held[0]['step']) == 2
+    for (ps, opt), h, m in zip(x.both(), held, moment):
+        opt.state[ps[1]] = h
+        opt.state[ps[2]]['exp_avg'] = m
+    x.step()
+    x.step()
+
+
+def test_replaced_states_that_do_not_fit_are_refused_and_lose_nothing(entries):
+    from pde_surrogate_amd import optim
+    ps = params(5, 300, 7)
+    opt = optim.FusedAdamW(ps)
+    grads(ps, 1)
+    opt.step()
+    good = copy.deepcopy(opt.state_dict())
+    weights = [p.detach().clone() for p in ps]
+    first, second = opt.state[ps[0]], opt.state[ps[1]]['exp_avg']
+    for change, match in ((lambda: opt.state[ps[1]].__setitem__('exp_avg', torch.zeros(7)), 'shape'),
+                          (lambda: opt.state[ps[1]].pop('exp_avg_sq'), 'exp_avg_sq'), (lambda: opt.state[ps[1]].pop('step'), "'step'")):
+        opt.state[ps[0]] = {k: v.clone() for k, v in first.items()}          # replaced as well, and fine
+        kept = dict(opt.state[ps[1]])
+        change()
+        for _ in range(2):
+            with pytest.raises(ValueError, match=match):
+                opt.step()
+        opt.state[ps[1]] = kept
+        opt.state[ps[1]]['exp_avg'] = second
+    assert all(torch.equal(p, w) for p, w in zip(ps, weights))
+    now = opt.state_dict()
+    assert all(torch.equal(now['state'][k][n], good['state'][k][n]) for k in range(3) for n in good['state'][k])
+    other = optim.FusedAdamW(copy.deepcopy(ps))
+    other.load_state_dict(good)
+    for o in (opt, other):
+        grads(o.param_groups[0]['params'], 2)
+        o.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, other.param_groups[0]['params']))
+
+
+def test_host_functions_on_states():
+    """note and held: dictionaries that are changed and changed back, entries of the program's own, tensors that get other memory"""
+    from pde_surrogate_amd.adamw import _host, _words
+    host = _host()
+    ps = params(3, 4)
+    buf = torch.zeros(20)
+    state = {p: {'step': torch.tensor(1.0), 'a': buf[5 * k:5 * k + 5]} for k, p in enumerate(ps)}
+    known = [x for p in ps for x in (p, state[p], 'step', state[p]['step'], 'a', state[p]['a'], None)]
+    dicts, tensors = [state[p] for p in ps], [state[p][k] for p in ps for k in ('step', 'a')]
+    note, at = _words(1 + 2 + 8)
+    host.note(state, dicts, tensors, at)
+
+    def held():
+        return host.held(state, known, dicts, tensors, at)
+    assert held() and held()
+    state[ps[1]]['mine'] = 3                       # entries of the program's own, in a state and beside them
+    state['other'] = {}
+    assert held() and held()
+    keep = state[ps[0]]['a']
+    state[ps[0]]['a'] = keep.clone()
+    assert not held() and not held()
+    state[ps[0]]['a'] = keep
+    assert held()
+    keep.data = keep.data.clone()
+    assert not held()
+    keep.data = buf[0:5]
+    assert held()
+    keep.data = buf[1:6]
+    assert not held()
+    keep.data = buf[0:5]
+    for change, back in ((lambda: state.__setitem__(ps[0], dict(dicts[0])), lambda: state.__setitem__(ps[0], dicts[0])),
+                         (lambda: state.__setitem__(ps[0], None), lambda: state.__setitem__(ps[0], dicts[0])),
+                         (lambda: state[ps[1]].pop('step'), None), ):
+        change()
+        assert not held()
+        if back:
+            back()
+            assert held()
+    state[ps[1]] = {'step': known[10], 'a': known[12]}
+    del state[ps[0]]
+    assert not held()
+    for bad in (lambda: host.held(state, known, dicts, tensors), lambda: host.held([], known, dicts, tensors, at), lambda: host.held(state, (), dicts, tensors, at),
+                lambda: host.note(state, [3], [], at), lambda: host.note(state, [], [3], at), lambda: host.note(state, [], ())):
+        with pytest.raises(TypeError):
+            bad()
