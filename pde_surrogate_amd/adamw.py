@@ -241,6 +241,7 @@ class _Plan:
 
     def __init__(self, launches, groups):
         self.launches = launches
+        self.stretches = [(x.ptr_at, x.size_at, x.count, x.params[0].element_size()) for x in launches]
         self.groups, self.counts = list(groups), [len(g['params']) for g in groups]
         self.params = [p for g in groups for p in g['params']]
         self.mask = bytes(p.grad is not None for p in self.params)
@@ -482,6 +483,7 @@ class FusedAdamW(torch.optim.Optimizer):
         same = self._holds()
         if not same:
             self._sift()
+        # (_gather asks this of every step; here it is asked before states are made)
         if _overlap([(p.data_ptr(), p.numel() * p.element_size()) for _, p, _ in active]):
             raise RuntimeError('FusedAdamW: two parameters share their memory')
         new = [p for _, p, _ in active if p not in self._where]
@@ -582,6 +584,9 @@ class FusedAdamW(torch.optim.Optimizer):
         for x in plan.launches:
             if host.gather(x.params, x.like, x.state.dtype, self._device.index, x.size_at, x.ptr_at, x.grad_at) != -1:
                 kept += self._gather_slowly(x)
+        # workgroups of one launch would read and write the same elements
+        if host.overlap(plan.stretches):
+            raise RuntimeError('FusedAdamW: two parameters share their memory')
         return kept
 
     def _reorder(self):

@@ -119,6 +119,42 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// overlap(lists) -> whether two stretches of memory have bytes in common.  lists: tuples (address of an array of addresses, of one
+// of numbers of elements, how many, bytes of an element)
+PyObject* overlap(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 1 || !as_list(args[0])) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "overlap takes a list");
+      return nullptr;
+    }
+    std::vector<std::pair<unsigned long long, unsigned long long>> used;         // first byte, byte behind the last
+    bool sorted = true;
+    for (Py_ssize_t j = 0; j < PyList_GET_SIZE(args[0]); ++j) {
+      const unsigned long long *at, *size;
+      Py_ssize_t count;
+      int item;
+      if (!PyTuple_Check(PyList_GET_ITEM(args[0], j))) {
+        PyErr_SetString(PyExc_TypeError, "overlap takes a list of tuples");
+        return nullptr;
+      }
+      unsigned long long a, b;
+      if (!PyArg_ParseTuple(PyList_GET_ITEM(args[0], j), "KKni", &a, &b, &count, &item)) return nullptr;
+      at = reinterpret_cast<const unsigned long long*>(a);
+      size = reinterpret_cast<const unsigned long long*>(b);
+      used.reserve(used.size() + count);
+      for (Py_ssize_t k = 0; k < count; ++k)
+        if (size[k]) {
+          sorted = sorted && (used.empty() || used.back().first <= at[k]);
+          used.emplace_back(at[k], at[k] + size[k] * item);
+        }
+    }
+    if (!sorted) std::sort(used.begin(), used.end());
+    for (size_t k = 1; k < used.size(); ++k)
+      if (used[k].first < used[k - 1].second) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
+  });
+}
+
 // fits(groups, params, mask) -> whether the lists of parameters in `groups` are, one behind the other, these very objects, and
 // those with a gradient are the ones that `mask` (bytes) marks
 PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -271,6 +307,7 @@ PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gradients)), METH_FASTCALL, nullptr},
+    {"overlap", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(overlap)), METH_FASTCALL, nullptr},
     {"fits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fits)), METH_FASTCALL, nullptr},
     {"note", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(note)), METH_FASTCALL, nullptr},
     {"held", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(held)), METH_FASTCALL, nullptr},

@@ -280,3 +280,57 @@ def test_host_functions_on_states():
                 lambda: host.note(state, [3], [], at), lambda: host.note(state, [], [3], at), lambda: host.note(state, [], ())):
         with pytest.raises(TypeError):
             bad()
+
+
+# ---- parameters that come to share memory ---------------------------------------------------------------------------------
+def test_parameters_that_share_memory_after_a_step_are_refused(entries):
+    from pde_surrogate_amd import optim
+    ps = params(*[30 + k for k in range(12)])
+    opt = optim.FusedAdamW([{'params': [p], 'lr': 1e-3 * (k + 1)} for k, p in enumerate(ps)])        # two launches
+    grads(ps, 1)
+    opt.step()
+    assert entries.launches == [8, 4]
+    whole = torch.randn(200)
+    for a, b, mine, other in ((0, 1, slice(0, 30), slice(29, 60)), (0, 11, slice(50, 80), slice(40, 81)), (5, 7, slice(0, 35), slice(0, 37)),
+                              (9, 2, slice(0, 39), slice(38, 70))):
+        keep = ps[a].data, ps[b].data
+        ps[a].data, ps[b].data = whole[mine], whole[other]
+        before, states = whole.clone(), [x.clone() for x in opt.flat_state()['exp_avg']]
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match='share their memory'):
+                opt.step()
+        assert torch.equal(whole, before) and all(torch.equal(x, y) for x, y in zip(states, opt.flat_state()['exp_avg']))
+        assert float(opt.state[ps[a]]['step']) == 1 and len(entries.launches) == 2
+        ps[a].data, ps[b].data = keep
+    for k, p in enumerate(ps):                     # one behind the other without a gap, in any order
+        at = (7 * k % 12) * 50
+        p.data = torch.zeros(600)[at:at + 30 + k]
+    opt.step()
+    flat = torch.zeros(sum(p.numel() for p in ps))
+    at = flat.numel()
+    for p in ps:
+        p.data = flat[at - p.numel():at]
+        at -= p.numel()
+    opt.step()
+    assert float(opt.state[ps[3]]['step']) == 3
+
+
+def test_stretches_of_memory():
+    from pde_surrogate_amd.adamw import _host, _words
+
+    def overlap(*lists):
+        made = []
+        for item, stretches in lists:
+            (at, x), (n, y) = _words(len(stretches)), _words(len(stretches))
+            for k, (start, size) in enumerate(stretches):
+                at[k], n[k] = start, size
+            made.append((x, y, len(stretches), item, at, n))
+        return _host().overlap([m[:4] for m in made])
+    assert not overlap() and not overlap((4, [])) and not overlap((4, [(8, 1), (12, 3), (24, 1)]))
+    assert overlap((4, [(8, 1), (12, 3), (20, 1)])) and overlap((4, [(8, 4), (8, 4)])) and overlap((4, [(40, 1), (8, 9)]))
+    assert not overlap((4, [(40, 1), (8, 8), (0, 0), (20, 0), (41, 0)])) and not overlap((2, [(40, 1), (8, 16)])) and overlap((2, [(40, 1), (8, 17)]))
+    assert overlap((4, [(0, 1), (100, 1)]), (2, [(50, 2), (102, 1)])) and not overlap((4, [(0, 1), (100, 1)]), (2, [(50, 2), (104, 1)]))
+    assert overlap((4, [((1 << 47) + 4, 1 << 39), (1 << 47, 2)])) and not overlap((4, [((1 << 47) + 4, 1 << 39), (1 << 47, 1)]))
+    for bad in (lambda: _host().overlap(()), lambda: _host().overlap([3]), lambda: _host().overlap([(1, 2)]), lambda: _host().overlap()):
+        with pytest.raises(TypeError):
+            bad()
