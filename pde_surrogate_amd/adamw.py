@@ -326,6 +326,10 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f'Invalid epsilon value: {group["eps"]}')
         if not 0.0 <= group['weight_decay']:
             raise ValueError(f'Invalid weight_decay value: {group["weight_decay"]}')
+        if bool(group.get('maximize', self.maximize)) != self.maximize:
+            raise ValueError(f'a group with maximize={group["maximize"]}: all groups go the same way (an argument of the constructor)')
+        if group.get('amsgrad'):
+            raise ValueError('amsgrad is not supported')
         for p in group['params']:
             _check_tensor(p, 'a parameter')
             if not _dense(p):
@@ -439,6 +443,8 @@ class FusedAdamW(torch.optim.Optimizer):
         sd = super().state_dict()
         # here parameters that are stepped together share one count; another optimiser would count it once for each of them
         sd['state'] = {k: {**v, 'step': v['step'].clone()} if 'step' in v else v for k, v in sd['state'].items()}
+        for g in sd['param_groups']:       # (where torch.optim.AdamW keeps it)
+            g['maximize'] = self.maximize
         if self.state_bits == 8:           # whose blocks belong to stretches of memory, whatever the shape
             for k, p in enumerate(p for g in self.param_groups for p in g['params']):
                 if 'step' in sd['state'].get(k, ()):

@@ -334,3 +334,46 @@ def test_stretches_of_memory():
     for bad in (lambda: _host().overlap(()), lambda: _host().overlap([3]), lambda: _host().overlap([(1, 2)]), lambda: _host().overlap()):
         with pytest.raises(TypeError):
             bad()
+
+
+# ---- saving and loading ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('ours', [False, True])
+def test_the_direction_is_part_of_a_saved_state(entries, ours):
+    from pde_surrogate_amd import optim
+    ps, qs, rs = params(5, 30), params(5, 30), params(5, 30)
+    a, b = optim.FusedAdamW(ps, maximize=ours), optim.FusedAdamW(qs, maximize=not ours)
+    grads(ps, 1)
+    grads(qs, 1)
+    a.step()
+    b.step()
+    keep = {k: v.clone() for k, v in b.state[qs[0]].items()}
+    with pytest.raises(ValueError, match='maximize'):
+        b.load_state_dict(a.state_dict())
+    assert all(torch.equal(b.state[qs[0]][k], v) for k, v in keep.items())
+    other = torch.optim.AdamW(rs, maximize=not ours)
+    other.load_state_dict(copy.deepcopy(a.state_dict()))
+    assert [g['maximize'] for g in other.param_groups] == [ours]
+    for p, r in zip(ps, rs):
+        r.data.copy_(p.data)
+    for x, o in ((ps, a), (rs, other)):
+        grads(x, 2)
+        o.step()
+    assert all(float((p - r).detach().abs().max()) <= 40 * 2.0 ** -24 * (1e-2 + float(p.detach().abs().max())) for p, r in zip(ps, rs))
+    assert a.state_dict()['param_groups'][0]['maximize'] is ours
+    # dictionaries without the entry, as they were saved before it was written, are taken as the optimiser's own
+    sd = a.state_dict()
+    del sd['param_groups'][0]['maximize']
+    a.load_state_dict(sd)
+
+
+def test_groups_with_choices_of_their_own_that_do_not_exist_are_refused(entries):
+    from pde_surrogate_amd import optim
+    ps = params(5, 6)
+    for extra in (dict(maximize=True), dict(amsgrad=True)):
+        with pytest.raises(ValueError, match=next(iter(extra))):
+            optim.FusedAdamW([{'params': ps[:1]}, {'params': ps[1:], **extra}])
+        opt = optim.FusedAdamW(ps[:1])
+        with pytest.raises(ValueError, match=next(iter(extra))):
+            opt.add_param_group({'params': ps[1:], **extra})
+        assert len(opt.param_groups) == 1
+    optim.FusedAdamW([{'params': ps, 'maximize': True, 'amsgrad': False}], maximize=True)
