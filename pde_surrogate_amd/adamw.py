@@ -440,7 +440,14 @@ class FusedAdamW(torch.optim.Optimizer):
         self._reset()
 
     def state_dict(self):
-        sd = super().state_dict()
+        # between the base class and the program's own hooks, which see what is returned
+        hook = self.register_state_dict_post_hook(FusedAdamW._complete, prepend=True)
+        try:
+            return super().state_dict()
+        finally:
+            hook.remove()
+
+    def _complete(self, sd):
         # here parameters that are stepped together share one count; another optimiser would count it once for each of them
         sd['state'] = {k: {**v, 'step': v['step'].clone()} if 'step' in v else v for k, v in sd['state'].items()}
         for g in sd['param_groups']:       # (where torch.optim.AdamW keeps it)
@@ -449,21 +456,26 @@ class FusedAdamW(torch.optim.Optimizer):
             for k, p in enumerate(p for g in self.param_groups for p in g['params']):
                 if 'step' in sd['state'].get(k, ()):
                     sd['state'][k]['order'] = _order(self._where[p][2] if p in self._where else p)
-        return sd
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        saved, groups = state_dict['state'], state_dict['param_groups']
-        if any(g.get('amsgrad') for g in groups):
-            raise ValueError('load_state_dict: amsgrad states are not supported')
-        if any(bool(g.get('maximize', self.maximize)) != self.maximize for g in groups):
-            raise ValueError(f'load_state_dict: maximize is {not self.maximize} in the dictionary and {self.maximize} here (a choice of the constructor)')
-        ours, theirs = [p for g in self.param_groups for p in g['params']], [i for g in groups for i in g['params']]
-        before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_retired', '_where', '_arenas', '_plan')}
+        before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_retired', '_where', '_arenas', '_plan', '_known')}
         steps = [st['step'] for st in self.state.values() if 'step' in st]
-        try:
+        taken = {}
+
+        def take(_, sd):                   # behind the program's own hooks, which may replace the dictionary
+            groups = sd['param_groups']
+            if any(g.get('amsgrad') for g in groups):
+                raise ValueError('load_state_dict: amsgrad states are not supported')
+            if any(bool(g.get('maximize', self.maximize)) != self.maximize for g in groups):
+                raise ValueError(f'load_state_dict: maximize is {not self.maximize} in the dictionary and {self.maximize} here (a choice of the constructor)')
+            taken.update(sd)
             # the base class would convert the states to their parameters' type: it gets the groups alone
-            super().load_state_dict({'state': {}, 'param_groups': groups})
+            return {**sd, 'state': {}}
+
+        def fill(_):                       # before the program's own hooks, which see the states
+            ours, theirs = [p for g in self.param_groups for p in g['params']], [i for g in taken['param_groups'] for i in g['params']]
+            saved = taken['state']
             self.state = defaultdict(dict, {p: dict(saved[i]) for i, p in zip(theirs, ours) if saved.get(i)})
             for p, st in self.state.items():
                 if tuple(st.pop('order', _order(p))) != _order(p):
@@ -472,11 +484,18 @@ class FusedAdamW(torch.optim.Optimizer):
                 self._check_group(g)
             with _lib.device_guard(self._device):
                 self._make_states(list(self.state))
+            self._retired = before['_retired']
+            self._retire(before['_arenas'], steps)
+
+        hooks = self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(fill, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
         except Exception:                  # an optimiser that cannot take the dictionary is left as it was
             self.__dict__.update(before)
             raise
-        self._retired = before['_retired']
-        self._retire(before['_arenas'], steps)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     # -- the step --------------------------------------------------------------------------------------------------------
     def _build(self, capturing):

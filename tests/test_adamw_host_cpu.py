@@ -377,3 +377,54 @@ def test_groups_with_choices_of_their_own_that_do_not_exist_are_refused(entries)
             opt.add_param_group({'params': ps[1:], **extra})
         assert len(opt.param_groups) == 1
     optim.FusedAdamW([{'params': ps, 'maximize': True, 'amsgrad': False}], maximize=True)
+
+
+def test_hooks_on_saving_and_loading(entries):
+    """as torch.optim documents them: a loading pre-hook sees the whole dictionary and may replace it, a post-hook sees the states that
+    were loaded, hooks on saving see what is returned"""
+    from pde_surrogate_amd import optim
+    ps, qs = params(5, 30), params(5, 30)
+    a, b = optim.FusedAdamW(ps), optim.FusedAdamW(qs)
+    grads(ps, 1)
+    a.step()
+    seen = []
+    a.register_state_dict_pre_hook(lambda o: seen.append('pre save'))
+
+    def saved(o, sd):
+        assert sd['state'][0]['step'] is not sd['state'][1]['step'] and sd['param_groups'][0]['maximize'] is False
+        sd['mine'] = 'something'
+        seen.append('post save')
+    a.register_state_dict_post_hook(saved)
+
+    def replaced(o, sd):
+        assert o is b and set(sd['state']) == {0, 1} and sd['state'][0]['exp_avg'].shape == (5,) and sd['mine'] == 'something'
+        seen.append('pre load')
+        return {**sd, 'state': {0: {**sd['state'][0], 'exp_avg': sd['state'][0]['exp_avg'] * 2}, 1: sd['state'][1]}}
+    b.register_load_state_dict_pre_hook(replaced)
+
+    def loaded(o):
+        assert torch.equal(o.state[qs[0]]['exp_avg'], a.state[ps[0]]['exp_avg'] * 2) and torch.equal(o.state[qs[1]]['exp_avg'], a.state[ps[1]]['exp_avg'])
+        assert len(o.flat_state()['exp_avg']) == 1
+        seen.append('post load')
+    b.register_load_state_dict_post_hook(loaded)
+    sd = a.state_dict()
+    assert set(sd) == {'state', 'param_groups', 'mine'}
+    for _ in range(2):
+        b.load_state_dict(sd)
+    assert seen == ['pre save', 'post save'] + ['pre load', 'post load'] * 2
+    assert torch.equal(sd['state'][0]['exp_avg'], a.state[ps[0]]['exp_avg'])
+
+    # a dictionary that cannot be taken, or a hook that fails: the optimiser is as it was, and the next one is taken as before
+    grads(qs, 2)
+    b.step()
+    keep = [(k, {n: x.clone() for n, x in v.items()}) for k, v in b.state.items()]
+    bad = copy.deepcopy(sd)
+    bad['state'][1]['exp_avg'] = torch.zeros(3)
+    with pytest.raises(ValueError, match='shape'):
+        b.load_state_dict(bad)
+    with pytest.raises(KeyError):
+        b.load_state_dict({k: v for k, v in sd.items() if k != 'mine'})
+    assert all(torch.equal(b.state[p][n], x) for p, st in keep for n, x in st.items())
+    seen.clear()
+    b.load_state_dict(sd)
+    assert seen == ['pre load', 'post load'] and float(b.state[qs[0]]['step']) == 1
