@@ -449,7 +449,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _complete(self, sd):
         # here parameters that are stepped together share one count; another optimiser would count it once for each of them
-        sd['state'] = {k: {**v, 'step': v['step'].clone()} if 'step' in v else v for k, v in sd['state'].items()}
+        sd['state'] = {k: {**v, 'step': v['step'].clone()} if isinstance(v.get('step'), torch.Tensor) else v for k, v in sd['state'].items()}
         for g in sd['param_groups']:       # (where torch.optim.AdamW keeps it)
             g['maximize'] = self.maximize
         if self.state_bits == 8:           # whose blocks belong to stretches of memory, whatever the shape

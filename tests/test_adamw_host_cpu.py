@@ -428,3 +428,10 @@ def test_hooks_on_saving_and_loading(entries):
     seen.clear()
     b.load_state_dict(sd)
     assert seen == ['pre load', 'post load'] and float(b.state[qs[0]]['step']) == 1
+
+
+def test_a_dictionary_of_an_optimiser_whose_counts_are_numbers(entries):
+    x = Pair([5, 30])
+    x.step()
+    x.ours.state[x.ps[0]]['step'] = 7
+    assert x.ours.state_dict()['state'][0]['step'] == 7 and float(x.ours.state_dict()['state'][1]['step']) == 1
