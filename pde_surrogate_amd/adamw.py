@@ -482,8 +482,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     raise ValueError('load_state_dict: the 8-bit state of a parameter belongs to another memory order than it has')
             for g in self.param_groups:
                 self._check_group(g)
-            with _lib.device_guard(self._device):
-                self._make_states(list(self.state))
+            if self.state:                 # (groups without parameters have no device)
+                with _lib.device_guard(self._device):
+                    self._make_states(list(self.state))
             self._retired = before['_retired']
             self._retire(before['_arenas'], steps)
 

@@ -435,3 +435,11 @@ def test_a_dictionary_of_an_optimiser_whose_counts_are_numbers(entries):
     x.step()
     x.ours.state[x.ps[0]]['step'] = 7
     assert x.ours.state_dict()['state'][0]['step'] == 7 and float(x.ours.state_dict()['state'][1]['step']) == 1
+
+
+def test_an_optimiser_of_nothing_is_saved_and_loaded(entries):
+    from pde_surrogate_amd import optim
+    a, b = optim.FusedAdamW([{'params': [], 'lr': 0.5}]), optim.FusedAdamW([{'params': []}])
+    b.load_state_dict(a.state_dict())
+    b.step()
+    assert b.param_groups[0]['lr'] == 0.5
