@@ -416,13 +416,12 @@ class FusedAdamW(torch.optim.Optimizer):
             st = self.state.get(p)
             if not (st and 'step' in st and all(st.get(name) is view and view.data_ptr() == at for name, view, at in views)):
                 del self._where[p]
-        used = {id(where[0]) for where in self._where.values()}
-        self._retire([a for a in self._arenas if id(a) not in used])
-        self._arenas = [a for a in self._arenas if id(a) in used]
 
     def flat_state(self):
-        """{name: [the flat buffers that hold this state, one per element type]}: the parameters' states one behind the other
-        in the order of the parameter list, each from a multiple of 256 elements on ('..._scale': one value per 256)"""
+        """{name: [the flat buffers that hold this state]}: one per element type, the parameters' states one behind the other in
+        the order of the parameter list, each from a multiple of 256 elements on ('..._scale': one value per 256).  States that
+        were made in a later step, replaced by the program or brought into another memory order follow in buffers of their own; the
+        place that such a state had before holds what was there"""
         out = {}
         for arena in self._arenas:
             for name, buf in arena.bufs.items():
@@ -515,6 +514,9 @@ class FusedAdamW(torch.optim.Optimizer):
         new = [p for _, p, _ in active if p not in self._where]
         if new:
             self._make_states(new)
+        used = {id(where[0]) for where in self._where.values()}
+        self._retire([a for a in self._arenas if id(a) not in used])
+        self._arenas = [a for a in self._arenas if id(a) in used]
         # a class: a group's parameters of one arena at the same step.  They share one count, which the call increments once.
         # On the device the values are unknown: there, what has shared a count so far goes on sharing it
         holders, classes, values, counts = {}, {}, {}, {}

@@ -443,3 +443,40 @@ def test_an_optimiser_of_nothing_is_saved_and_loaded(entries):
     b.load_state_dict(a.state_dict())
     b.step()
     assert b.param_groups[0]['lr'] == 0.5
+
+
+# ---- memory ---------------------------------------------------------------------------------------------------------------
+def _buffers(opt):
+    return [len(v) for v in opt.flat_state().values()]
+
+
+def test_buffers_of_states_that_have_moved_are_dropped(entries):
+    from pde_surrogate_amd import optim
+    import gc
+    import weakref
+    ps = [torch.nn.Parameter(torch.randn(8, 6, 3, 3)), torch.nn.Parameter(torch.randn(77))]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    a, b = optim.FusedAdamW(ps), optim.FusedAdamW(qs)
+    gone = []
+    for t in range(8):
+        grads(qs, t)
+        ps[0].grad = None
+        ps[0].data = ps[0].data.to(memory_format=torch.channels_last if t % 2 else torch.contiguous_format)
+        for p, q in zip(ps, qs):
+            p.grad = q.grad.clone()
+        a.step()
+        b.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+        # the first buffers, in which the second parameter's states still are, and one more of each
+        assert _buffers(a) == [1 if t == 0 else 2] * 2
+        gone.append([weakref.ref(x[-1]) for x in a.flat_state().values()])
+    gc.collect()
+    assert [x[0]() is None and x[1]() is None for x in gone] == [False] + [True] * 6 + [False]
+    # a state that is taken out again and again, and all of them at once
+    for t in range(6):
+        a.state[ps[1]] = {}
+        a.step()
+        assert _buffers(a) == [2] * 2
+    a.state.clear()
+    a.step()
+    assert _buffers(a) == [1] * 2 and float(a.state[ps[0]]['step']) == 1
