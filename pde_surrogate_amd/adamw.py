@@ -272,7 +272,8 @@ class FusedAdamW(torch.optim.Optimizer):
     belong to stretches of the parameter's memory, so a parameter keeps the order of its dimensions there for good.
 
     A graph captured from a step holds the states it was captured with: capture again after load_state_dict, and after a step
-    in which other parameters had gradients.  Memory that such a graph may write to is kept for as long as the optimiser."""
+    in which other parameters had gradients or states were replaced.  The states and counts that such a graph writes to are kept for as
+    long as the optimiser."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
                  clip_norm=None, maximize=False, capturable=False, seed=0):
@@ -285,7 +286,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.maximize = state_bits, bool(master_weights), bool(maximize)
         self.clip_norm, self.capturable, self.seed = None if clip_norm is None else float(clip_norm), bool(capturable), int(seed)
         self.grad_norm = None
-        self._retired = []
+        self._captured = {}         # what captured steps work on, by identity: graphs may write to it after it has been replaced
         self._reset()
         self._device = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -296,11 +297,6 @@ class FusedAdamW(torch.optim.Optimizer):
         self._arenas = []
         self._plan = None
         self._known = None          # the states as the last plan found or made them (see _holds)
-
-    def _retire(self, *what):
-        """a captured graph may still write to buffers that have been replaced: they stay until the optimiser goes"""
-        if self.capturable:
-            self._retired.extend(what)
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -435,7 +431,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self.grad_norm = None
-        self._retired = []
+        self.__dict__.setdefault('_captured', {})
         self._reset()
 
     def state_dict(self):
@@ -458,8 +454,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_retired', '_where', '_arenas', '_plan', '_known')}
-        steps = [st['step'] for st in self.state.values() if 'step' in st]
+        before = {k: self.__dict__[k] for k in ('state', 'param_groups', 'grad_norm', '_where', '_arenas', '_plan', '_known')}
         taken = {}
 
         def take(_, sd):                   # behind the program's own hooks, which may replace the dictionary
@@ -484,8 +479,6 @@ class FusedAdamW(torch.optim.Optimizer):
             if self.state:                 # (groups without parameters have no device)
                 with _lib.device_guard(self._device):
                     self._make_states(list(self.state))
-            self._retired = before['_retired']
-            self._retire(before['_arenas'], steps)
 
         hooks = self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(fill, prepend=True)
         try:
@@ -515,7 +508,6 @@ class FusedAdamW(torch.optim.Optimizer):
         if new:
             self._make_states(new)
         used = {id(where[0]) for where in self._where.values()}
-        self._retire([a for a in self._arenas if id(a) not in used])
         self._arenas = [a for a in self._arenas if id(a) in used]
         # a class: a group's parameters of one arena at the same step.  They share one count, which the call increments once.
         # On the device the values are unknown: there, what has shared a count so far goes on sharing it
@@ -544,7 +536,6 @@ class FusedAdamW(torch.optim.Optimizer):
         counted = {}
         for key, (arena, g, step, members) in classes.items():
             if holders.get(id(step)) != len(members):      # (the program may hold the count of a state that it has replaced)
-                self._retire(step)
                 step = step.clone()
             for _, _, _, _, st in members:
                 st['step'] = step
@@ -622,7 +613,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if self.state_bits == 8:
             raise RuntimeError('FusedAdamW: a parameter has another memory order than its 8-bit state')
         for p in [p for p, (_, _, like, _) in self._where.items() if not _same_order(p, like)]:
-            self._retire(self._where.pop(p), self.state[p])
+            del self._where[p]
 
     def _fits(self, plan):
         groups, lists = self.param_groups, [g['params'] for g in self.param_groups]
@@ -672,6 +663,13 @@ class FusedAdamW(torch.optim.Optimizer):
                 for _, _, count in x.classes:
                     count += 1
             host.changed(x.params, False)
-            if x.arena.stream != stream and not capturing:      # freed later than this stream's work on them
-                for buf in x.arena.bufs.values():
-                    buf.record_stream(torch.cuda.current_stream(device))
+            if capturing:
+                self._captured.update((id(kept), kept) for kept in [x.arena] + [t for g, step, _ in x.classes for t in (step, g['lr'])])
+            # what is replaced later is freed later than this stream's work on it
+            if not capturing:
+                if x.arena.stream != stream:
+                    for buf in x.arena.bufs.values():
+                        buf.record_stream(torch.cuda.current_stream(device))
+                for _, step, count in x.classes:
+                    if count is None:                               # (on the device)
+                        step.record_stream(torch.cuda.current_stream(device))

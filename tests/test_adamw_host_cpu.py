@@ -480,3 +480,39 @@ def test_buffers_of_states_that_have_moved_are_dropped(entries):
     a.state.clear()
     a.step()
     assert _buffers(a) == [1] * 2 and float(a.state[ps[0]]['step']) == 1
+
+
+def test_a_changing_set_of_gradients_keeps_nothing(entries):
+    """with counts on the device as well: only what a captured step works on is kept beside the states"""
+    from pde_surrogate_amd import optim
+    import gc
+    import weakref
+    ps = params(5, 30, 7)
+    opt = optim.FusedAdamW(ps, capturable=True)
+    counts = []
+    for t in range(12):
+        grads(ps, t, which=(0, 1, 2) if t % 2 else (0, t // 2 % 3))
+        opt.step()
+        counts += [weakref.ref(opt.state[p]['step']) for p in ps if p in opt.state]
+    gc.collect()
+    alive = {id(x()) for x in counts if x() is not None}
+    assert alive == {id(opt.state[p]['step']) for p in ps}
+    assert [float(opt.state[p]['step']) for p in ps] == [12, 8, 8]
+
+    # a captured step's counts and buffers stay (the stand-in computes at once what a graph would compute when it is replayed)
+    grads(ps, 0)
+    opt.step()
+    entries.capturing = True
+    opt.step()
+    entries.capturing = False
+    kept = [weakref.ref(x) for x in [opt.state[p]['step'] for p in ps] + [x for v in opt.flat_state().values() for x in v]]
+    opt.load_state_dict(opt.state_dict())
+    opt.state.clear()
+    grads(ps, 1, which=(1,))
+    opt.step()
+    gc.collect()
+    assert all(x() is not None for x in kept)
+    late = [weakref.ref(x) for x in [opt.state[ps[1]]['step']] + [x for v in opt.flat_state().values() for x in v]]
+    opt.load_state_dict(opt.state_dict())
+    gc.collect()
+    assert all(x() is None for x in late) and all(x() is not None for x in kept)
