@@ -588,8 +588,9 @@ int pdes_multi_dot(const float* W, long long ld, int rows, const float* V, int n
  * Operators over a LIST of tensors (no reference counterpart; torch.optim.AdamW and torch.nn.utils.clip_grad_norm_ are the
  * interfaces behind which pde_surrogate_amd/adamw.py puts them).  `params`, `grads`: host arrays of device addresses, aligned
  * to the element only, each tensor dense; everything that describes the list is read at call time and passed to the kernels by
- * value.  Lists of any length (a launch takes 96 or 160 tensors), tensors of 0 to 2^40 - 1 elements.  All tensors of a call
- * have one element type; several calls make a mixed list. */
+ * value.  Lists of any length (a launch takes 96 or 160 tensors), tensors of 0 to 2^40 - 1 elements, under 2^40 together.  All
+ * tensors of a call have one element type; several calls make a mixed list.  What a call writes has no memory in common with
+ * anything else that it reads or writes (not checked).  A list is refused before any of its launches. */
 enum { PDES_MT_F32 = 0, PDES_MT_BF16 = 1, PDES_MT_F16 = 2 };
 #define PDES_MT_BLOCK 256    /* elements that share a scale of 8-bit states; every tensor's state starts at a multiple */
 #define PDES_MT_CLASSES 8    /* hyper-parameter sets of one pdes_adamw_step call */

@@ -516,3 +516,21 @@ def test_a_changing_set_of_gradients_keeps_nothing(entries):
     opt.load_state_dict(opt.state_dict())
     gc.collect()
     assert all(x() is None for x in late) and all(x() is not None for x in kept)
+
+
+# ---- the C entries --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('at', [159, 160, 161, 400])
+def test_a_bad_entry_anywhere_in_a_list_is_refused_before_anything_is_launched(at):
+    """every call is rejected on the host (a launch takes 160 tensors, and the ones in front are fine)"""
+    import ctypes
+    from pde_surrogate_amd import _lib
+    L = _lib.lib()
+    for address, size, want in ((0, 10, -1), (4098, 10, -3), (4096, -1, -1), (4096, 1 << 40, -1)):
+        grads_, sizes = (ctypes.c_ulonglong * 401)(*[4096] * 401), (ctypes.c_longlong * 401)(*[10] * 401)
+        grads_[at], sizes[at] = address, size
+        assert L.pdes_grad_norm(grads_, sizes, 401, 0, 2, 4096, 0, None) == want
+        assert L.pdes_clip_grads(grads_, sizes, 401, 0, 2, 4096, 1.0, 4096, None) == want
+        # without a limit nothing is read, and the list is checked all the same
+        assert L.pdes_clip_grads(grads_, sizes, 401, 0, 2, 4096, float('inf'), 4096, None) == want
+    sizes = (ctypes.c_longlong * 401)(*[1 << 32] * 401)                  # 2^40 and more together
+    assert L.pdes_grad_norm((ctypes.c_ulonglong * 401)(*[4096] * 401), sizes, 401, 0, 2, 4096, 0, None) == -1
