@@ -267,7 +267,9 @@ class FusedAdamW(torch.optim.Optimizer):
 
     A gradient of another memory order than its parameter's is copied into the parameter's first; every parameter has to be
     dense, and no two may share memory.  Parameters without a gradient are left out of a step, as in torch.  `amsgrad`, sparse
-    and complex parameters are not offered.  A gradient that is not finite spoils the elements it belongs to and no others.
+    and complex parameters are not offered.  A gradient that is not finite spoils the elements it belongs to and no others,
+    unless a finite clip_norm lets it into the common factor: an infinite norm makes that 0 (all other gradients count as zeros in
+    that step), a NaN makes it NaN, and with it every parameter, as torch's clipping and step do.
     With 8-bit states eps under 2^-100 counts as 2^-100, and blocks whose largest value is under that are held as zeros; they
     belong to stretches of the parameter's memory, so a parameter keeps the order of its dimensions there for good.
 

@@ -369,7 +369,8 @@ __device__ __forceinline__ void step32(typename T::E* p, const typename T::E* g,
     if constexpr (LOW) { lo[0] = (int16_t)lw[u][0]; lo[1] = (int16_t)(lw[u][0] >> 16); lo[2] = (int16_t)lw[u][1]; lo[3] = (int16_t)(lw[u][1] >> 16); }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float gk = T::up(ge[u][k]) * gf;
+      // (a factor that is NaN stays out of the padding)
+      const float gk = !ALL && k >= left ? 0.f : T::up(ge[u][k]) * gf;
       mv[u][k] = mv[u][k] * h.b1 + gk * h.ob1;
       vv[u][k] = vv[u][k] * h.b2 + gk * gk * h.ob2;
       pe[u][k] = narrow<T, LOW>(new_weight(widen<T, LOW>(pe[u][k], lo[k]), mv[u][k], sqrtf(vv[u][k]), h), lo[k]);
@@ -538,7 +539,9 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
   bool small = false;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float gk = CLIP ? T::up(ge[k]) * gf : T::up(ge[k]);
+    // (a factor that is NaN stays out of the padding)
+    const bool there = ALL || k % Share<T>::PER + k / Share<T>::PER * Share<T>::APART < cnt;
+    const float gk = !CLIP ? T::up(ge[k]) : there ? T::up(ge[k]) * gf : 0.f;
     m[k] = m[k] * h.b1 + gk * h.ob1;
     v[k] = r[k] * r[k] * h.b2 + gk * gk * h.ob2;
     r[k] = EXACT ? root(v[k]) : near_root(v[k]);
