@@ -635,7 +635,8 @@ typedef struct pdes_adamw_state {
 /* One AdamW step (decoupled weight decay, bias correction, eps outside the root):
  *   g = factor * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   w = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32, one rounding per operation; gradients are left as they are.  The elements of the state buffers behind a tensor's
+ * in fp32, one rounding per operation (with bits 8, bf16 / fp16 parameters without `low` are computed with fused sums and an
+ * approximate reciprocal, a few 2^-24 of the change off, before they are rounded); gradients are left as they are.  The elements of the state buffers behind a tensor's
  * last element, up to its block's end, stay zero if they were. */
 int pdes_adamw_step(const unsigned long long* params, const unsigned long long* grads, const pdes_mt_tensor* tensors,
                     int count, const pdes_adamw_class* classes, int nclasses, const pdes_adamw_state* state, void* stream);

@@ -7,7 +7,7 @@
 Any list of fp32, bf16 or fp16 parameters on one GPU takes part, whichever module they belong to: `optim.Adam` needs one HIP
 network's flat buffer for its one-launch step, `FusedAdamW` takes the tensors as they are, up to 96 in a launch.  The
 kernels are csrc/multi_tensor.hip; the arithmetic is fp32 with one rounding per operation (include/pdes_hip.h:
-pdes_adamw_step), the norm's sum is fp64 in a fixed order, so equal inputs give equal bits.
+pdes_adamw_step, and the one exception), the norm's sum is fp64 in a fixed order, so equal inputs give equal bits.
 """
 import ctypes
 import math

@@ -6,8 +6,9 @@
 // earlier launch still reads it, and a captured graph holds its own copy.
 //
 // This file is compiled with -ffp-contract=off: every product and sum below rounds once, in the order written, so that a
-// step on equal inputs gives equal bits whichever kernel, chunk or launch an element falls into, and the 8-bit codes and the
-// kept low halves can be compared exactly with any other computation of the same formulas.
+// step on equal inputs gives equal bits whichever kernel, chunk or launch an element falls into, and the moments, the 8-bit codes
+// and the kept low halves can be compared exactly with any other computation of the same formulas.  One exception: with 8-bit states
+// the new value of a 16-bit weight without a low half (new_weight_16).
 #include <math.h>
 #include "pdes_common.h"
 #include "../../include/pdes_hip.h"
@@ -449,24 +450,15 @@ __device__ __forceinline__ void unpack8(uint32_t w, float scale, float* x) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
   x[0] = a[0] * scale; x[1] = a[1] * scale; x[2] = b[0] * scale; x[3] = b[1] * scale;
 }
-// sqrtf, correctly rounded for x >= 2^-96: the hardware's root is off by one place at most, and the signs of x - s s' for its
-// two neighbours s' say which of the three is nearest.  (What sqrtf does besides is scaling for small x.  There the result is
-// off by a place at most, and subnormal x go through sqrtf itself.)  0, infinity and NaN come out as they are: the neighbours'
-// residuals are NaN or zero and change nothing.
+// sqrtf, correctly rounded, for x = 0 and 2^-102 <= x < infinity: from the reciprocal root and one correction by the residual.  (All
+// 2^24 numbers of two neighbouring binades have been compared with sqrtf, at 2^0, 2^-60 and 2^-100; four times the number gives
+// exactly twice the root.  Under 2^-102 the residual loses bits.)  NaN for infinity
 __device__ __forceinline__ float root(float x) {
-  const float s = __builtin_amdgcn_sqrtf(x);
-  const float under = __uint_as_float(__float_as_uint(s) - 1u), over = __uint_as_float(__float_as_uint(s) + 1u);
-  float r = fmaf(-under, s, x) <= 0.f ? under : s;
-  return fmaf(-over, s, x) > 0.f ? over : r;
-}
-// The same but for one in two million x, where the result is the neighbour: from the reciprocal root (off by a place) and one
-// correction by the residual, whose own error is 2^-22 of a place.  Not for infinity and subnormal numbers.
-__device__ __forceinline__ float near_root(float x) {
   const int bits = __float_as_int(x), least = 0x00800000;                      // (2^-126; x is not negative)
   const float y = __builtin_amdgcn_rsqf(__int_as_float(bits > least ? bits : least)), s = x * y;
   return fmaf(fmaf(-s, s, x), 0.5f * y, s);
 }
-constexpr int ODD_ROOT = 0x290;              // class mask: subnormal numbers and infinity
+constexpr uint32_t ROOT_LEAST = 0x0f800000u;                                   // 2^-96 as bits
 
 // A half wave holds a block, a lane eight elements of it: consecutive ones of 16 bits, or twice four of 32 bits, 128 elements
 // apart, so that each access of a wave covers whole lines (332 M fp32 parameters, streaming: 852 us; eight consecutive ones, two
@@ -520,7 +512,8 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
                                       long long cnt, float gf, const MtHyper& h, uint32_t key, int lane) {
   // Weights of 16 bits leave 10 bytes of traffic per element, about the time of this arithmetic.  There the weight itself is
   // computed with fused sums and the reciprocal instruction, off by a few places of 2^-24 before it is rounded by 2^-9 or 2^-12.
-  // The moments are always held to the last place: which of two codes a value gets depends on it, and so do later scales.
+  // The moments are the same numbers for every type: which of two codes a value gets depends on their last place, and so do
+  // later scales.
   constexpr bool EXACT = sizeof(typename T::E) == 4 || LOW;
   typename T::E pe[8], ge[8];
   int16_t lw[8] = {};
@@ -536,7 +529,7 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
   float m[8], r[8], v[8];
   unpack8(mw[0], m_scale, m); unpack8(mw[1], m_scale, m + 4);
   unpack8(rw[0], r_scale, r); unpack8(rw[1], r_scale, r + 4);
-  bool small = false;
+  uint32_t mtop = 0, rtop = 0, least = ~0u;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     // (a factor that is NaN stays out of the padding)
@@ -544,21 +537,25 @@ __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, 
     const float gk = !CLIP ? T::up(ge[k]) : there ? T::up(ge[k]) * gf : 0.f;
     m[k] = m[k] * h.b1 + gk * h.ob1;
     v[k] = r[k] * r[k] * h.b2 + gk * gk * h.ob2;
-    r[k] = EXACT ? root(v[k]) : near_root(v[k]);
-    small |= __builtin_amdgcn_classf(v[k], ODD_ROOT);
+    r[k] = root(v[k]);
+    const uint32_t mb = __float_as_uint(m[k]) & 0x7fffffffu, rb = __float_as_uint(r[k]), vb = __float_as_uint(v[k]) - 1u;
+    mtop = mb > mtop ? mb : mtop;
+    rtop = rb > rtop ? rb : rtop;              // (r is not negative; a NaN with the sign is the largest as well)
+    least = vb < least ? vb : least;           // (of those that are not zero)
   }
-  if (small) {
+  if (least < ROOT_LEAST - 1u || rtop >= 0x7f800000u) {      // numbers that root() is not for; for the others sqrtf is the same
+    rtop = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) r[k] = sqrtf(v[k]);
+    for (int k = 0; k < 8; ++k) {
+      r[k] = sqrtf(v[k]);
+      const uint32_t rb = __float_as_uint(r[k]);
+      rtop = rb > rtop ? rb : rtop;
+    }
   }
-  uint32_t mtop = 0, rtop = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float w = widen<T, LOW>(pe[k], lw[k]);
     pe[k] = narrow<T, LOW>(EXACT ? new_weight(w, m[k], r[k], h) : new_weight_16(w, m[k], r[k], h), lw[k]);
-    const uint32_t mb = __float_as_uint(m[k]) & 0x7fffffffu, rb = __float_as_uint(r[k]);
-    mtop = mb > mtop ? mb : mtop;
-    rtop = rb > rtop ? rb : rtop;              // (r is not negative; a NaN with the sign is the largest as well)
   }
   store8<T, ALL, NT>(p, cnt, pe);
   if constexpr (LOW) {

@@ -60,3 +60,55 @@ def test_a_norm_that_is_not_finite(dev, bits, dtype, master):
             for name, bufs in a.flat_state().items():
                 if not name.endswith('_scale'):
                     assert not bufs[0].view(torch.uint8).view(bufs[0].numel(), -1)[_padding(bufs[0], sizes)].any(), (name, bad, t)
+
+
+@pytest.mark.parametrize('dtype,master', [('float32', False), ('bfloat16', False), ('bfloat16', True)])
+def test_roots_of_very_small_second_moments(dev, dtype, master):
+    """Gradients of 1e-18 to 1e-14, whose squares times 1e-3 are subnormal or a little above: the 8-bit states are their definition's, bit
+    for bit, whatever their neighbours are (a lane works on eight elements at once, and roots of small numbers take another way)"""
+    from pde_surrogate_amd import optim
+    rng = np.random.default_rng(11)
+    n = 256 * 3000
+    mag = 10.0 ** rng.uniform(-18, -14, (n // 256, 1)) * np.exp(rng.uniform(-0.3, 0, (n // 256, 256)))     # (blocks of one size: their tops show)
+    mag[::3, ::16] = 1e-21                                 # subnormal second moments among the others
+    mag[1::3, ::32] = 0.0
+    g = torch.from_numpy((mag * rng.choice([-1, 1], mag.shape)).astype(np.float32).reshape(-1)).to(DT[dtype]).to(dev)
+    p = torch.nn.Parameter(torch.zeros(n, dtype=DT[dtype], device=dev))
+    lr, betas, eps, wd, seed = 1e-3, (0.9, 0.999), 1e-8, 0.0, 3
+    opt = optim.FusedAdamW([p], lr=lr, betas=betas, eps=eps, weight_decay=wd, state_bits=8, master_weights=master, seed=seed)
+    blocks = n // 256
+    q = [np.zeros((blocks, 256), np.float32), np.zeros(blocks, np.float32)] * 2
+    for t in (1, 2):
+        p.grad = g * t
+        _, _, mc, ms, rc, rs = au.step8(np.zeros(n, np.float32), au.f64(p.grad).astype(np.float32), *q, t, lr, betas, eps, wd, seed, 0)
+        opt.step()
+        st = opt.state[p]
+        for name, want in (('exp_avg_scale', ms), ('rms_scale', rs)):
+            got = st[name].cpu().numpy()
+            assert np.array_equal(got, want), f'{name}, step {t}: {int((got != want).sum())} of {blocks} differ'
+        for name, want in (('exp_avg_q', mc), ('rms_q', rc)):
+            got = st[name].view(torch.uint8).cpu().numpy().reshape(want.shape)
+            assert np.array_equal(got, want), f'{name}, step {t}: {int((got != want).sum())} codes differ'
+        q = [x for a in ('exp_avg', 'rms') for x in (st[a + '_q'].float().cpu().numpy().reshape(blocks, 256), st[a + '_scale'].cpu().numpy())]
+
+
+@pytest.mark.parametrize('dtype,master', [('float32', False), ('bfloat16', False), ('bfloat16', True), ('float16', False)])
+def test_roots_of_many_second_moments(dev, dtype, master):
+    """Each of 2^18 blocks holds one element that is not zero, so that its scale is its root times 1 / 448: the scales of three steps are
+    those of fp32 operations one by one"""
+    from pde_surrogate_amd import optim
+    blocks, b2 = 1 << 18, 0.999
+    p = torch.nn.Parameter(torch.zeros(blocks * 256, dtype=DT[dtype], device=dev))
+    p.grad = torch.zeros_like(p)
+    gen = torch.Generator(dev).manual_seed(2)
+    opt = optim.FusedAdamW([p], lr=0.0, betas=(0.9, b2), state_bits=8, master_weights=master, seed=1)
+    r = np.zeros(blocks, np.float32)
+    for t in range(1, 4):
+        p.grad[::256] = torch.randn(blocks, generator=gen, device=dev).to(DT[dtype])
+        opt.step()
+        g = p.grad[::256].float().cpu().numpy()
+        r = np.sqrt(r * r * np.float32(b2) + g * g * np.float32(1 - b2))
+        want = r * np.float32(1 / 448)
+        got = opt.state[p]['rms_scale'].cpu().numpy()
+        assert want.dtype == np.float32 and np.array_equal(got, want), f'step {t}: {int((got != want).sum())} of {blocks} scales differ'
+        r = opt.state[p]['rms_q'].view(blocks, 256)[:, 0].float().cpu().numpy() * got
