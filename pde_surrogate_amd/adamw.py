@@ -13,7 +13,6 @@ import ctypes
 import math
 from array import array
 from collections import defaultdict
-from operator import is_
 
 import torch
 
@@ -236,13 +235,17 @@ class _Reordered(Exception):
     """a parameter's memory has another order than its state's"""
 
 
+class _Ungraded(Exception):
+    """a parameter of the plan has no gradient any more"""
+
+
 class _Plan:
     """the launches of a step, for as long as the same parameters of the same groups have gradients and no state is replaced"""
 
     def __init__(self, launches, groups):
         self.launches = launches
         self.stretches = [(x.ptr_at, x.size_at, x.count, x.params[0].element_size()) for x in launches]
-        self.groups, self.counts = list(groups), [len(g['params']) for g in groups]
+        self.groups = [x for g in groups for x in (g, len(g['params']))]       # (the launches' constants come from these dictionaries)
         self.params = [p for g in groups for p in g['params']]
         self.mask = bytes(p.grad is not None for p in self.params)
 
@@ -559,6 +562,8 @@ class FusedAdamW(torch.optim.Optimizer):
         to be kept until the launch is enqueued), a parameter that has got another order itself needs its state in that order,
         everything else that the kernels cannot take is an error"""
         kept = []
+        if any(p.grad is None for p in launch.params):
+            raise _Ungraded
         for k, p in enumerate(launch.params):
             g, dtype = p.grad, launch.arena.dtype
             if g.layout != torch.strided:
@@ -589,12 +594,15 @@ class FusedAdamW(torch.optim.Optimizer):
             if capturing and not self.capturable:
                 raise RuntimeError('FusedAdamW: a step is captured into a graph only with capturable=True')
             plan = self._plan if self._plan is not None and self._fits(self._plan) else self._build(capturing)
-            try:
-                kept = self._gather(plan)
-            except _Reordered:
-                self._reorder()
-                plan = self._build(capturing)
-                kept = self._gather(plan)
+            kept = None
+            while kept is None:
+                try:
+                    kept = self._gather(plan)
+                except _Ungraded:
+                    plan = self._build(capturing)
+                except _Reordered:
+                    self._reorder()
+                    plan = self._build(capturing)
             self._run(plan, capturing)
             del kept
         return loss
@@ -618,11 +626,7 @@ class FusedAdamW(torch.optim.Optimizer):
             del self._where[p]
 
     def _fits(self, plan):
-        groups, lists = self.param_groups, [g['params'] for g in self.param_groups]
-        return (self._holds() and
-                # the plan's constants come from these dictionaries, whose parameters stand one behind the other in plan.params
-                len(groups) == len(plan.groups) and all(map(is_, groups, plan.groups)) and [len(x) for x in lists] == plan.counts and
-                _host().fits(lists, plan.params, plan.mask))
+        return _host().fits(self.param_groups, plan.params, plan.mask, plan.groups) and self._holds()
 
     def _run(self, plan, capturing):
         device, L, host = self._device, _lib.lib(), _host()
@@ -667,11 +671,11 @@ class FusedAdamW(torch.optim.Optimizer):
             host.changed(x.params, False)
             if capturing:
                 self._captured.update((id(kept), kept) for kept in [x.arena] + [t for g, step, _ in x.classes for t in (step, g['lr'])])
-            # what is replaced later is freed later than this stream's work on it
-            if not capturing:
+            else:                           # what is replaced later is freed later than this stream's work on it
                 if x.arena.stream != stream:
                     for buf in x.arena.bufs.values():
                         buf.record_stream(torch.cuda.current_stream(device))
-                for _, step, count in x.classes:
-                    if count is None:                               # (on the device)
-                        step.record_stream(torch.cuda.current_stream(device))
+                if self.capturable:
+                    for _, step, count in x.classes:
+                        if count is None:                           # (on the device)
+                            step.record_stream(torch.cuda.current_stream(device))

@@ -157,23 +157,33 @@ PyObject* overlap(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // fits(groups, params, mask) -> whether the lists of parameters in `groups` are, one behind the other, these very objects, and
 // those with a gradient are the ones that `mask` (bytes) marks
+// fits(groups, params, mask, known) -> the same of an optimiser's groups: they are the very dictionaries in `known` (a list of each
+// and its number of parameters), and whether the marked parameters still have a gradient is left to gather, which looks at them
 PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
-    if (nargs != 3 || !as_list(args[0]) || !as_list(args[1]) || !PyBytes_Check(args[2]) || PyBytes_GET_SIZE(args[2]) != PyList_GET_SIZE(args[1])) {
+    static PyObject* const name = PyUnicode_InternFromString("params");
+    PyObject* const known = nargs == 4 ? args[3] : nullptr;
+    if (nargs < 3 || nargs > 4 || !as_list(args[0]) || !as_list(args[1]) || !PyBytes_Check(args[2]) ||
+        PyBytes_GET_SIZE(args[2]) != PyList_GET_SIZE(args[1]) || (known && !as_list(known))) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "fits takes a list of lists, a list and as many bytes");
       return nullptr;
     }
     const char* mask = PyBytes_AS_STRING(args[2]);
     const Py_ssize_t n = PyList_GET_SIZE(args[1]);
     Py_ssize_t at = 0;
+    if (known && PyList_GET_SIZE(known) != 2 * PyList_GET_SIZE(args[0])) Py_RETURN_FALSE;
     for (Py_ssize_t j = 0; j < PyList_GET_SIZE(args[0]); ++j) {
       PyObject* group = PyList_GET_ITEM(args[0], j);
+      if (known) {
+        if (group != PyList_GET_ITEM(known, 2 * j) || !PyDict_Check(group) || !(group = PyDict_GetItemWithError(group, name))) Py_RETURN_FALSE;
+        if (!PyList_Check(group) || PyList_GET_SIZE(group) != PyLong_AsSsize_t(PyList_GET_ITEM(known, 2 * j + 1))) Py_RETURN_FALSE;
+      }
       if (!as_list(group)) return nullptr;
       for (Py_ssize_t k = 0; k < PyList_GET_SIZE(group); ++k, ++at) {
         PyObject* o = PyList_GET_ITEM(group, k);
-        if (at >= n || o != PyList_GET_ITEM(args[1], at) || !THPVariable_Check(o) ||
-            THPVariable_Unpack(o).grad().defined() != (mask[at] != 0))
-          Py_RETURN_FALSE;
+        if (at >= n || o != PyList_GET_ITEM(args[1], at)) Py_RETURN_FALSE;
+        if (known && mask[at]) continue;
+        if (!THPVariable_Check(o) || THPVariable_Unpack(o).grad().defined() != (mask[at] != 0)) Py_RETURN_FALSE;
       }
     }
     if (at != n) Py_RETURN_FALSE;
@@ -194,14 +204,13 @@ uint64_t version_of(PyObject* dict) {
   return 0;
 #endif
 }
-// a tensor's storage, which views of one buffer share, and its place there
-bool place_of(PyObject* o, unsigned long long (&at)[2]) {
-  if (!THPVariable_Check(o)) return false;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  if (t.layout() != at::kStrided || !t.has_storage()) return false;
-  at[0] = reinterpret_cast<unsigned long long>(t.unsafeGetTensorImpl()->unsafe_storage().unsafeGetStorageImpl());
-  at[1] = static_cast<unsigned long long>(t.storage_offset());
-  return true;
+// a tensor's storage, which views of one buffer share (0: it has none), and its place there
+struct Place {
+  unsigned long long storage, offset;
+};
+inline Place place_of(const at::Tensor& t) {
+  const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+  return {reinterpret_cast<unsigned long long>(impl->unsafe_storage().unsafeGetStorageImpl()), static_cast<unsigned long long>(impl->storage_offset())};
 }
 void note_versions(PyObject* state, PyObject* dicts, unsigned long long* note) {
   *note++ = version_of(state);
@@ -240,17 +249,18 @@ PyObject* note(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "note takes a dictionary, a list of them, a list of tensors and an address");
       return nullptr;
     }
-    unsigned long long *out = words(args[3]), place[2];
+    unsigned long long* out = words(args[3]);
     if (PyErr_Occurred()) return nullptr;
     note_versions(args[0], args[1], out);
     out += 1 + PyList_GET_SIZE(args[1]);
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(args[2]); ++k) {
-      if (!place_of(PyList_GET_ITEM(args[2], k), place)) {
-        PyErr_SetString(PyExc_TypeError, "note takes tensors with a storage");
+      if (!THPVariable_Check(PyList_GET_ITEM(args[2], k))) {
+        PyErr_SetString(PyExc_TypeError, "note takes a list of tensors");
         return nullptr;
       }
-      *out++ = place[0];
-      *out++ = place[1];
+      const Place place = place_of(THPVariable_Unpack(PyList_GET_ITEM(args[2], k)));
+      *out++ = place.storage;
+      *out++ = place.offset;
     }
     Py_RETURN_NONE;
   });
@@ -263,7 +273,7 @@ PyObject* held(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "held takes a dictionary, three lists and an address");
       return nullptr;
     }
-    unsigned long long *noted = words(args[4]), place[2];
+    unsigned long long* noted = words(args[4]);
     if (PyErr_Occurred()) return nullptr;
     const Py_ssize_t n = PyList_GET_SIZE(args[2]);
     bool same = noted[0] != 0 && version_of(args[0]) == noted[0];
@@ -273,13 +283,14 @@ PyObject* held(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       note_versions(args[0], args[2], noted);
     }
     const unsigned long long* at = noted + 1 + n;
-    // (the objects are all over the heap: 2,000 of them between other work take 15 us less when the next ones are on their way)
+    // (the objects are all over the heap: 2,000 of them between other work take 15 us less when the next ones are on their way;
+    // all of them are tensors, as note has made sure)
     const Py_ssize_t m = PyList_GET_SIZE(args[3]), ahead = 8;
     for (Py_ssize_t k = 0; k < m; ++k, at += 2) {
       if (k + 2 * ahead < m) __builtin_prefetch(PyList_GET_ITEM(args[3], k + 2 * ahead));
-      if (k + ahead < m && THPVariable_Check(PyList_GET_ITEM(args[3], k + ahead)))
-        __builtin_prefetch(THPVariable_Unpack(PyList_GET_ITEM(args[3], k + ahead)).unsafeGetTensorImpl());
-      if (!place_of(PyList_GET_ITEM(args[3], k), place) || place[0] != at[0] || place[1] != at[1]) Py_RETURN_FALSE;
+      if (k + ahead < m) __builtin_prefetch(THPVariable_Unpack(PyList_GET_ITEM(args[3], k + ahead)).unsafeGetTensorImpl());
+      const Place place = place_of(THPVariable_Unpack(PyList_GET_ITEM(args[3], k)));
+      if (place.storage != at[0] || place.offset != at[1]) Py_RETURN_FALSE;
     }
     Py_RETURN_TRUE;
   });

@@ -534,3 +534,19 @@ def test_a_bad_entry_anywhere_in_a_list_is_refused_before_anything_is_launched(a
         assert L.pdes_clip_grads(grads_, sizes, 401, 0, 2, 4096, float('inf'), 4096, None) == want
     sizes = (ctypes.c_longlong * 401)(*[1 << 32] * 401)                  # 2^40 and more together
     assert L.pdes_grad_norm((ctypes.c_ulonglong * 401)(*[4096] * 401), sizes, 401, 0, 2, 4096, 0, None) == -1
+
+
+def test_everything_at_once(entries):
+    """a gradient less, one more, another memory order, a moved parameter and a replaced moment before one step"""
+    x = Pair([5, 300, 7, 256, 64], groups=2)
+    for ps, opt in x.both():
+        ps[4].data = ps[4].data.view(8, 8)
+    x.step(which=(0, 1, 4))
+    for t in range(3):
+        for ps, opt in x.both():
+            ps[4].grad = None
+            ps[4].data = ps[4].data.t().contiguous().t() if t % 2 == 0 else ps[4].data.contiguous()
+            opt.param_groups[t % 2]['params'].append(opt.param_groups[1 - t % 2]['params'].pop(0))
+            opt.state[ps[1]]['exp_avg'] = opt.state[ps[1]]['exp_avg'] + 1
+        x.step(which=(1, 2 + t % 2, 4))
+        x.step()
