@@ -1,13 +1,15 @@
 """Build libpdes_hip.so (all HIP kernels + the C ABI) in-tree with hipcc for gfx950, and _tensor_list.so (host code that reads
-Python lists of tensors, against the installed torch's headers) with g++.
+Python lists of tensors, against the installed torch's headers) with g++.  Where torch is not installed the kernels' library is
+all that is built.
 
     python -m pde_surrogate_amd.build            # rebuild if any source is newer than the .so
     python -m pde_surrogate_amd.build --force
 
-The .so is git-ignored (history stays source-only) but travels with the gpurun snapshot.
+Both are git-ignored: the history stays source-only.
 hipcc cross-compiles gfx950 without a GPU.
 """
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -32,8 +34,12 @@ def headers():
     return glob.glob(os.path.join(CSRC, '*.h')) + glob.glob(os.path.join(CSRC, '*.inc')) + glob.glob(os.path.join(os.path.dirname(HERE), 'include', '*.h'))
 
 
+def has_torch():
+    return importlib.util.find_spec('torch') is not None
+
+
 def needs_host_build():
-    return not os.path.exists(HOST_LIB) or os.path.getmtime(HOST_SRC) > os.path.getmtime(HOST_LIB)
+    return has_torch() and (not os.path.exists(HOST_LIB) or os.path.getmtime(HOST_SRC) > os.path.getmtime(HOST_LIB))
 
 
 def needs_build():
@@ -58,7 +64,9 @@ def build(force=False, verbose=True):
         return LIB
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
     objs = []
-    host = subprocess.Popen(host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT) if force or needs_host_build() else None
+    host = None
+    if needs_host_build() or (force and has_torch()):
+        host = subprocess.Popen(host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     # one object per source, compiled in parallel, then linked: keeps rebuilds to seconds
     procs = []
     for src in sources():
@@ -70,20 +78,23 @@ def build(force=False, verbose=True):
             if verbose:
                 print(' '.join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+    failed = []
     for src, p in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
             sys.stderr.write(out.decode())
-            raise RuntimeError(f'hipcc failed on {src}')
+            failed.append(f'hipcc failed on {src}')
     if host is not None:
-        out, _ = host.communicate()
-        if host.returncode != 0:
-            sys.stderr.write(out.decode())
-            raise RuntimeError(f'{os.environ.get("CXX", "g++")} failed on {HOST_SRC}')
+        host_out, _ = host.communicate()
+    if failed:
+        raise RuntimeError('; '.join(failed))
     cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC'] + objs + ['-o', LIB]
     if verbose:
         print(' '.join(cmd), flush=True)
     subprocess.check_call(cmd)
+    if host is not None and host.returncode != 0:             # (the kernels' library is whole)
+        sys.stderr.write(host_out.decode())
+        raise RuntimeError(f'{os.environ.get("CXX", "g++")} failed on {HOST_SRC}')
     return LIB
 
 
