@@ -112,3 +112,48 @@ def test_roots_of_many_second_moments(dev, dtype, master):
         got = opt.state[p]['rms_scale'].cpu().numpy()
         assert want.dtype == np.float32 and np.array_equal(got, want), f'step {t}: {int((got != want).sum())} of {blocks} scales differ'
         r = opt.state[p]['rms_q'].view(blocks, 256)[:, 0].float().cpu().numpy() * got
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype,master', [('float32', False), ('bfloat16', False), ('bfloat16', True), ('float16', False)])
+def test_long_lists_step_as_short_ones(dev, bits, dtype, master):
+    """34 M elements in one step, clipped: streaming accesses, the norm from a launch of its own, several tiles a workgroup where the rules
+    say so.  The same tensors, a few at a time and not clipped, take none of these; with a clipping factor of exactly 1/2 and
+    gradients halved by hand both do the same arithmetic, and their places in the list are the same: equal bits"""
+    from pde_surrogate_amd import optim
+    sizes = [1_000_003 + 517 * k for k in range(31)] + [1, 2048, 255, 3_100_000]
+    assert sum(sizes) > 32 << 20
+    gen = torch.Generator(dev).manual_seed(8)
+    ps = [torch.nn.Parameter((torch.randn(n, generator=gen, device=dev) * 0.05).to(DT[dtype])) for n in sizes]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    a, b = (optim.FusedAdamW(x, lr=1e-2, weight_decay=0.1, state_bits=bits, master_weights=master, seed=6) for x in (ps, qs))
+    few = [list(range(k, min(k + 4, len(ps)))) for k in range(0, len(ps), 4)]
+    assert max(sum(sizes[k] for k in part) for part in few) < 6 << 20
+    for t in range(2):
+        g = [(torch.randn(n, generator=gen, device=dev) * 10.0 ** -(k % 3)).to(DT[dtype]) for k, n in enumerate(sizes)]
+        for x in g:
+            x[x.abs() < 2.0 ** -13] = 0                    # (halves of fp16's subnormal numbers would be rounded)
+        g[33].zero_()                                      # brings the norm to 8192, so that the factor is 1 / 8192 * 4096
+        left = 8192.0 ** 2 - sum(float(x.double().square().sum()) for x in g)
+        for i in range(20):
+            x = torch.tensor(math.sqrt(max(left, 0.0)) * (1 - 2.0 ** -8)).to(DT[dtype])
+            if float(x) < 2.0 ** -13:
+                break
+            g[33][i] = x
+            left -= float(x) ** 2
+        assert 0 <= left < 8192.0 ** 2 * 2.0 ** -30
+        for p, x in zip(ps, g):
+            p.grad = x
+        a.clip_norm = 4096.0
+        a.step()
+        assert float(a.grad_norm) == 8192.0 == float(optim.clip_grad_norm_(ps, math.inf))
+        for part in few:
+            for k, q in enumerate(qs):
+                q.grad = g[k] * 0.5 if k in part else None
+            b.step()
+        for k, (p, q) in enumerate(zip(ps, qs)):
+            assert torch.equal(p, q), (k, t)
+            assert float(a.state[p]['step']) == float(b.state[q]['step']) == t + 1
+            for name in a.state[p]:
+                if name != 'step':
+                    assert torch.equal(a.state[p][name].view(torch.uint8), b.state[q][name].view(torch.uint8)), (name, k, t)
