@@ -400,7 +400,8 @@ class FusedAdamW(torch.optim.Optimizer):
             for item in state.items():
                 if item[0] in names:
                     known += item
-                    tensors[id(item[1])] = item[1]
+                    if isinstance(item[1], torch.Tensor):      # (a count that the program has set may be a number)
+                        tensors[id(item[1])] = item[1]
             known.append(None)
         tensors = list(tensors.values())
         note, at = _words(1 + len(dicts) + 2 * len(tensors))

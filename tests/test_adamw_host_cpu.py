@@ -550,3 +550,43 @@ def test_everything_at_once(entries):
             opt.state[ps[1]]['exp_avg'] = opt.state[ps[1]]['exp_avg'] + 1
         x.step(which=(1, 2 + t % 2, 4))
         x.step()
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+def test_a_count_that_is_a_number_while_its_parameter_has_no_gradient(entries, capturable):
+    from pde_surrogate_amd import optim
+    ps = params(5, 30, 7)
+    opt = optim.FusedAdamW(ps, capturable=capturable)
+    grads(ps, 1)
+    opt.step()
+    opt.state[ps[2]]['step'] = 20
+    for t in range(2):
+        grads(ps, 2 + t, which=(0, 1))
+        opt.step()
+    assert opt.state[ps[2]]['step'] == 20
+    grads(ps, 4)
+    opt.step()
+    assert [float(opt.state[p]['step']) for p in ps] == [4, 4, 21]
+
+
+def test_copies_are_saved_and_loaded(entries):
+    """a copied and a pickled optimiser step, save and load as the one they come from"""
+    import pickle
+    from pde_surrogate_amd import optim
+    ps = params(5, 30)
+    a = optim.FusedAdamW(ps)
+    grads(ps, 1)
+    a.step()
+    for x, b in (copy.deepcopy((ps, a)), pickle.loads(pickle.dumps((ps, a)))):
+        sd = b.state_dict()
+        assert all(torch.equal(sd['state'][k]['exp_avg'], a.state[p]['exp_avg']) for k, p in enumerate(ps))
+        b.load_state_dict(a.state_dict())
+        keep = [p.detach().clone() for p in ps]
+        c = optim.FusedAdamW(ps)
+        c.load_state_dict(a.state_dict())
+        for opt, y in ((b, x), (c, ps)):
+            grads(y, 2)
+            opt.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, x))
+        for p, k in zip(ps, keep):
+            p.data.copy_(k)
