@@ -22,6 +22,7 @@ BLOCK = 256                   # PDES_MT_BLOCK: every tensor's state starts at a 
 _CLASSES = 8                  # PDES_MT_CLASSES
 _ROWS = 256                   # PDES_MT_ROWS
 _HYPER_BYTES = 288            # PDES_MT_HYPER_BYTES
+_LARGEST = 2.0 ** 128 - 2.0 ** 104            # the largest fp32 number
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -110,6 +111,11 @@ def _words(n):
     return a, a.buffer_info()[0]
 
 
+def _limit(x):
+    """a limit as fp32: only infinity is none"""
+    return x if x == math.inf else min(x, _LARGEST)
+
+
 def _norm_rows(lists, kind, device, stream):
     """pdes_grad_norm over [(element type, address of the addresses, address of the sizes, how many)]"""
     rows = torch.empty(_ROWS, dtype=torch.float64, device=device)
@@ -163,7 +169,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
                                    'error_if_nonfinite=False they are multiplied by the factor that it gives')
         if max_norm != math.inf:
             for x in lists:
-                clip(*x, max_norm)
+                clip(*x, _limit(max_norm))
             _host().changed(params, True)
     return norm
 
@@ -645,7 +651,7 @@ class FusedAdamW(torch.optim.Optimizer):
             st = x.state
             st.bits, st.maximize, st.seed = self.state_bits, self.maximize, self.seed
             if rows is not None:
-                st.norm_rows, st.norm_out, st.limit = rows.data_ptr(), norm.data_ptr(), self.clip_norm
+                st.norm_rows, st.norm_out, st.limit = rows.data_ptr(), norm.data_ptr(), _limit(self.clip_norm)
             else:
                 st.norm_rows = None
             if self.capturable:

@@ -157,3 +157,25 @@ def test_long_lists_step_as_short_ones(dev, bits, dtype, master):
             for name in a.state[p]:
                 if name != 'step':
                     assert torch.equal(a.state[p][name].view(torch.uint8), b.state[q][name].view(torch.uint8)), (name, k, t)
+
+
+@pytest.mark.parametrize('inside', [False, True])
+def test_limits_beyond_fp32(dev, inside):
+    """a limit that fp32 does not hold is a limit all the same: only infinity means none.  With an infinite norm the factor is 0"""
+    from pde_surrogate_amd import optim
+    for limit, factor in ((1e39, 0.0), (1e300, 0.0), (math.inf, 1.0)):
+        ps = [torch.nn.Parameter(torch.zeros(5, device=dev)) for _ in range(2)]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        ps[1].grad[2] = math.inf
+        if inside:
+            opt = optim.FusedAdamW(ps, lr=1.0, weight_decay=0.0, clip_norm=limit)
+            opt.step()
+            got, norm = opt.state[ps[0]]['exp_avg'] / np.float32(1 - 0.9), opt.grad_norm
+        else:
+            norm = optim.clip_grad_norm_(ps, limit)
+            got = ps[0].grad
+        assert float(norm) == math.inf and (got == factor).all()
+    ps[1].grad[2] = 1.0
+    ps[0].grad.fill_(1.0)
+    assert float(optim.clip_grad_norm_(ps, 1e39)) == np.float32(math.sqrt(10)) and (ps[0].grad == 1).all()
