@@ -1,5 +1,7 @@
 // Operators over many tensors in one launch: the AdamW step with 32-bit or 8-bit states, the common norm of a list of
-// gradients, and their clipping (include/pdes_hip.h: pdes_adamw_step, pdes_grad_norm, pdes_clip_grads).
+// gradients, and their clipping (include/pdes_hip.h: pdes_adamw_step, pdes_grad_norm, pdes_clip_grads).  Where a comment compares
+// two ways, both were built from this file and timed in turn on one MI355X; 332 M and 217 M
+// are 332,410,880 and 216,545,280 elements, any other M is 2^20.
 //
 // The list is cut into chunks, each inside one tensor; a workgroup of a step takes one.  The list itself (addresses, lengths) travels BY VALUE in the
 // kernel arguments, up to 96 tensors a launch: nothing to copy, no buffer that a later call could overwrite while an
@@ -122,8 +124,8 @@ __device__ __forceinline__ void put(void* p, W w, int k = 0) {
   else *q = w;
 }
 // N consecutive elements.  ALL: they exist; otherwise `cnt` of them do (the others read as zero and are not written).  The
-// whole-vector form is a plain global access without a branch, so that a thread's loads are all under way at once (fp32 norm
-// of 332 M elements: 368 us with a branch at each load, 222 us without)
+// whole-vector form is a plain global access without a branch, so that a thread's loads are all under way at once (norm of 332 M
+// fp32 elements: 224 us with a branch at each load, 195 without; fp16 121 and 102)
 template <class T, int N, bool ALL, bool NT>
 __device__ __forceinline__ void load(const typename T::E* p, long long cnt, typename T::E (&x)[N]) {
   typedef typename T::E E;
@@ -226,7 +228,8 @@ __device__ __forceinline__ void norm_chunk(const typename T::E* g, long long lef
     }
 }
 // One workgroup a CU and row; a thread has U accesses of 16 bytes under way.  Bound by reading: 332 M elements of fp32 192 us =
-// 6.9 TB/s, of bf16 98 us = 6.8 TB/s (streaming), 214 and 113 us through the caches.
+// 6.9 TB/s, of bf16 99 us = 6.7 TB/s (a call 195 and 101 us; 216 and 114 through the caches).  The maximum norm compares in fp64,
+// three instructions an element: 197 and 117 us.
 template <class T, int KIND, int THREADS, int U, bool NT>
 __global__ __launch_bounds__(THREADS) void grad_norm_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(typename T::E), CHUNK = THREADS * V * U;
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(MT_ROWS) void norm_kernel(const double* rows, float
   if (threadIdx.x == 0) *norm = x;
 }
 
-// gradients times the clipping factor; where that is 1 nothing is read or written
+// Gradients times the clipping factor; where that is 1 nothing is read or written.  332 M elements of fp32 483 us, of bf16 240 us, both
+// 5.5 TB/s (half of it writes); 20 M fp32, found in the cache by the norm in front, 26 us.
 template <class T, bool ALL>
 __device__ __forceinline__ void clip_chunk(typename T::E* g, long long left, float f) {
   constexpr int V = 16 / sizeof(typename T::E), TILE = 256 * V;
@@ -461,8 +465,8 @@ __device__ __forceinline__ float root(float x) {
 constexpr uint32_t ROOT_LEAST = 0x0f800000u;                                   // 2^-96 as bits
 
 // A half wave holds a block, a lane eight elements of it: consecutive ones of 16 bits, or twice four of 32 bits, 128 elements
-// apart, so that each access of a wave covers whole lines (332 M fp32 parameters, streaming: 852 us; eight consecutive ones, two
-// accesses to each half of a line: 975 us).
+// apart, so that each access of a wave covers whole lines (332 M fp32 parameters: 886 us; eight consecutive ones, two accesses to
+// each half of a line: 1,130 us).
 template <class T>
 struct Share {
   static constexpr int PER = sizeof(typename T::E) == 4 ? 4 : 8, PARTS = 8 / PER, APART = 128;
@@ -510,10 +514,10 @@ __device__ __forceinline__ void put_codes(uint8_t* q, u32x2 w) {
 template <class T, bool LOW, bool CLIP, bool NT, bool ALL>
 __device__ __forceinline__ void step8(typename T::E* p, const typename T::E* g, uint8_t* mq, uint8_t* rq, float* ms, float* rs, int16_t* low,
                                       long long cnt, float gf, const MtHyper& h, uint32_t key, int lane) {
-  // Weights of 16 bits leave 10 bytes of traffic per element, about the time of this arithmetic.  There the weight itself is
-  // computed with fused sums and the reciprocal instruction, off by a few places of 2^-24 before it is rounded by 2^-9 or 2^-12.
-  // The moments are the same numbers for every type: which of two codes a value gets depends on their last place, and so do
-  // later scales.
+  // Weights of 16 bits leave 10 bytes of traffic per element (332 M bf16: 562 us = 5.9 TB/s), about the time of this arithmetic.
+  // There the weight itself is computed with fused sums and the reciprocal instruction, off by a few places of 2^-24 before it is
+  // rounded by 2^-9 or 2^-12.  The moments are the same numbers for every type: which of two codes a value gets depends on their
+  // last place, and so do later scales.
   constexpr bool EXACT = sizeof(typename T::E) == 4 || LOW;
   typename T::E pe[8], ge[8];
   int16_t lw[8] = {};
@@ -672,11 +676,11 @@ __global__ __launch_bounds__(64) void adamw_count_kernel(const ClassArgs a) {
 }
 
 constexpr long long LONG_LIST = 8ll << 20;
-// Tiles of a workgroup.  One, so that the workgroups walk through memory side by side (332 M fp32 elements: 1,749 us, with four
-// 1,790; 8-bit states: 919 and 1,011).  16-bit elements with 8-bit states, where a workgroup's start (table, keys, clipping factor)
-// weighs more: two from 8 M elements on, and four from 32 M on with clipping, whose factor each workgroup loads first (bf16 elements
-// with one / two / four: 332 M 587 / 570 / 620 us; 4 M 10.2 / 10.2 / 13; clipped, with the norm, 332 M 752 / 697 / 694, 150 M with
-// low halves 440 / 429 / 422, 16 M 47 / 43 / 44)
+// Tiles of a workgroup.  One, so that the workgroups walk through memory side by side (8-bit states of 332 M fp32 elements: 886 us,
+// with two 937, with four 978).  16-bit elements with 8-bit states, where a workgroup's start (table, keys, clipping factor) weighs
+// more: two from 8 M elements on, and four from 32 M on with clipping, whose factor each workgroup loads first (us with one / two /
+// four: bf16 8 M 19.6 / 17.2 / 18.3, 64 M 117 / 117 / 134, 332 M 564 / 563 / 618; with low halves 332 M 839 / 795 / 834; clipped, with
+// the norm, bf16 16 M 42.7 / 41.4 / 40.6, 64 M 159 / 141 / 139, 332 M 754 / 682 / 700, with low halves 150 M 459 / 431 / 425)
 static uint32_t tiles_of(int bits, int size, bool clip, long long total) {
   if (bits == 32 || size == 4 || total < LONG_LIST) return 1;
   return clip && total >= 4 * LONG_LIST ? 4 : 2;
@@ -711,10 +715,11 @@ static int fill(NormArgs& a, const unsigned long long* grads, const long long* s
   return taken;
 }
 
-// Lists up to 4 MiB, a pass of the chip: 256 threads and chunks of 16 KiB (0.7 M fp32 elements 3.8 us; 5.8 us with the others'
-// shape).  Longer ones: 1024 threads and 64 KiB.  Streaming from 512 MiB on, twice the last-level cache: under it the optimiser's
-// step that follows finds part of the gradients there (norm and step of 100 M fp32 elements: 525 us, streaming 535; from 300 M
-// elements on streaming is the faster by a per cent, and by a tenth for the norm alone).
+// Lists up to 4 MiB, a pass of the chip: 256 threads and chunks of 16 KiB (0.7 M fp32 elements 3.2 us, 3.7 with the others' shape).
+// Longer ones: 1024 threads and 64 KiB (332 M fp32: 196 us, 264 with the short ones' shape).  Streaming from 512 MiB on, twice the
+// last-level cache: under it the optimiser's step that follows finds part of the gradients there (norm and step of fp32 elements,
+// cached and streaming: 64 M 350 and 362 us, 100 M 545 and 555; from 200 M on both take the same, and the norm alone is faster by a
+// tenth).
 constexpr int LONG_THREADS = 1024, SHORT_THREADS = 256, NORM_U = 4;
 constexpr long long SHORT_MOST = 16ll * MT_ROWS * SHORT_THREADS * NORM_U, NORM_STREAMS = 512ll << 20;
 template <class T, int KIND>
@@ -740,12 +745,18 @@ static void launch_clip(int kind, const NormArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((clip_kernel<T, 0>), dim3(grid), dim3(256), 0, st, a);
 }
 
-// Streaming accesses for steps that touch more than this: with less, parts are still in the 256 MiB cache at the next step
-// (8 M fp32 elements = 122 MiB: 41 us streaming, 46 not; 4 M: 22 and 18).
+// Streaming accesses for steps that touch more than this.  With less, parts are still in the 256 MiB cache at the next step; with
+// more, the rest of a training step has put other data there.  Four lists stepped in turn, through the caches and streaming (us):
+//   32-bit states  fp32 4 M (64 MiB) 20.4 and 22.6, 6 M (96 MiB) 37.1 and 32.0, 16 M 92.2 and 78.4; bf16 6 M (72 MiB) 26.0 and 26.9,
+//                  8 M (96 MiB) 37.6 and 34.6; low halves 4 M 18.6 and 22.2, 8 M (112 MiB) 45.6 and 40.9; fp16 as bf16
+//   8-bit states   fp32 8 M (80 MiB) 27.4 and 24.9, 12 M (120 MiB) 40.6 and 35.3; bf16 8 M (48 MiB) 17.9 and 17.6, 16 M (96 MiB) 37.0
+//                  and 32.4; low halves 8 M (64 MiB) 25.3 and 25.2, 12 M (96 MiB) 38.7 and 34.8; fp16 as bf16
+// (One list alone, stepped again and again with nothing between, would stay cached up to 256 MiB: fp32 8 M 35.7 and 41.8.)
 constexpr long long STEP_STREAMS = 96ll << 20;
 // Streaming steps with 32-bit states run best with two (fp32) or three (16-bit) workgroups on a CU, 64 to 84 KiB of loads under
-// way: the memory keeps fewer pages open (332 M fp32 elements: 1,529 us with two, 1,571 with three, 1,603 with four, 1,645
-// with the seven that the registers allow; bf16: 1,184 us with three, 1,270 with seven, 1,335 with two).  Unused LDS holds the others off.
+// way: the memory keeps fewer pages open (us with two / three / four / as many as the registers allow: 332 M fp32 1,505 / 1,564 / 1,601 /
+// 1,637; bf16 1,317 / 1,166 / 1,208 / 1,308, fp16 the same; 217 M with low halves 962 / 956 / 983 / 1,019).  Unused LDS holds the
+// others off.
 constexpr unsigned HOLD_TWO = 80000, HOLD_THREE = 53000;
 template <class T, bool LOW, bool NT>
 static void launch_step(int bits, const StepArgs& a, hipStream_t st) {
@@ -868,8 +879,9 @@ extern "C" int pdes_adamw_step(const unsigned long long* params, const unsigned 
   a.m = s.exp_avg; a.v = s.exp_avg_sq; a.ms = s.exp_avg_scale; a.rs = s.rms_scale; a.low = s.low;
   a.limit = s.limit;
   if (clip && total > LONG_LIST) {
-    // every workgroup of a step can add up the rows by itself, which saves a launch (1 M elements with 8-bit states: 10.6 us for
-    // norm and step, 13.5 with the launch); where they are many, that costs more (64 M: 219 us, 210 with the launch)
+    // every workgroup of a step can add up the rows by itself, which saves a launch (1 M elements: 21.7 us a call for norm and step,
+    // 24.6 with the launch); where they are many, that costs as much or more (200 M: fp32 with 8-bit states 683 us, 673 with the
+    // launch; bf16 with 32-bit states 833 and 816; at 64 M both are within a per cent)
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(MT_ROWS), 0, st, a.rows, a.norm);
     PDES_LAUNCH_CHECK();
     a.rows = nullptr;

@@ -1,8 +1,7 @@
 """The build: the kernels' library needs hipcc alone; _tensor_list.so needs the installed torch's headers and is left out where
 there is no torch.  The compilers are stand-ins that write what they were called with."""
-import os
+import importlib.util
 import stat
-import sys
 
 import pytest
 
@@ -54,9 +53,12 @@ def test_everything_is_built_once(tree):
 
 def test_without_torch_the_kernels_are_built(tree, monkeypatch):
     build, path, calls = tree
-    for name in [k for k in sys.modules if k == 'torch' or k.startswith('torch.')]:
-        monkeypatch.delitem(sys.modules, name)
-    monkeypatch.setitem(sys.modules, 'torch', None)                   # `import torch` raises ImportError, and so does find_spec
+    real = importlib.util.find_spec
+
+    def none():
+        raise ModuleNotFoundError("No module named 'torch'")
+    monkeypatch.setattr(importlib.util, 'find_spec', lambda name, *a: None if name == 'torch' else real(name, *a))
+    monkeypatch.setattr(build, 'host_command', none)                  # (which imports it)
     for force in (False, True):
         build.build(force=force, verbose=False)
         got = calls()
