@@ -179,3 +179,30 @@ def test_limits_beyond_fp32(dev, inside):
     ps[1].grad[2] = 1.0
     ps[0].grad.fill_(1.0)
     assert float(optim.clip_grad_norm_(ps, 1e39)) == np.float32(math.sqrt(10)) and (ps[0].grad == 1).all()
+
+
+@pytest.mark.parametrize('dtype', ['bfloat16', 'float16'])
+def test_8_bit_states_of_16_bit_weights_are_their_definition(dev, dtype):
+    """codes and scales bit for bit, as for fp32 weights (the weights themselves: one rounding of 16 bits, test_adamw_gpu.py)"""
+    from pde_surrogate_amd import optim
+    sizes = [1_500_007, 255, 1, 8192, 300_000]
+    gen = torch.Generator().manual_seed(17)
+    ps = [torch.nn.Parameter((torch.randn(n, generator=gen) * 0.05).to(DT[dtype]).to(dev)) for n in sizes]
+    lr, betas, eps, wd, seed = 2e-3, (0.9, 0.95), 1e-8, 0.1, 5
+    opt = optim.FusedAdamW(ps, lr=lr, betas=betas, eps=eps, weight_decay=wd, state_bits=8, seed=seed)
+    for t in range(1, 4):
+        before = []
+        for k, p in enumerate(ps):
+            p.grad = (torch.randn(sizes[k], generator=gen) * 10.0 ** -k).to(DT[dtype]).to(dev)
+            st, blocks = opt.state.get(p, {}), -(-sizes[k] // au.BLOCK)
+            before.append([x for a in ('exp_avg', 'rms') for x in (
+                (st[a + '_q'].float().cpu().numpy().reshape(blocks, au.BLOCK), st[a + '_scale'].cpu().numpy()) if st
+                else (np.zeros((blocks, au.BLOCK), np.float32), np.zeros(blocks, np.float32)))])
+        opt.step()
+        for k, p in enumerate(ps):
+            _, _, mc, ms, rc, rs = au.step8(np.zeros(sizes[k], np.float32), au.f64(p.grad).astype(np.float32), *before[k], t, lr, betas, eps, wd, seed, k)
+            st = opt.state[p]
+            for name, want in (('exp_avg_q', mc), ('rms_q', rc)):
+                got = st[name].view(torch.uint8).cpu().numpy().reshape(want.shape)
+                assert np.array_equal(got, want), f'{name} of tensor {k}, step {t}: {int((got != want).sum())} codes differ'
+            assert np.array_equal(st['exp_avg_scale'].cpu().numpy(), ms) and np.array_equal(st['rms_scale'].cpu().numpy(), rs), (k, t)
