@@ -204,7 +204,7 @@ def device_guard(device):
     """make `device` current for the launches inside (streams, events and kernels of a call all belong to the device of
     its tensors); free when it already is"""
     import torch
-    idx = torch.device(device).index
+    idx = device.index if isinstance(device, torch.device) else torch.device(device).index
     if idx is None or idx == torch.cuda.current_device():
         return _NOGUARD
     return torch.cuda.device(idx)
