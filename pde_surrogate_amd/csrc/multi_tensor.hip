@@ -228,8 +228,8 @@ __device__ __forceinline__ void norm_chunk(const typename T::E* g, long long lef
     }
 }
 // One workgroup a CU and row; a thread has U accesses of 16 bytes under way.  Bound by reading: 332 M elements of fp32 192 us =
-// 6.9 TB/s, of bf16 99 us = 6.7 TB/s (a call 195 and 101 us; 216 and 114 through the caches).  The maximum norm compares in fp64,
-// three instructions an element: 197 and 117 us.
+// 6.9 TB/s, of bf16 99 us = 6.7 TB/s (a call 195 and 101 us; 216 and 114 through the caches).  The maximum norm has three fp64
+// comparisons an element: 197 and 117 us.
 template <class T, int KIND, int THREADS, int U, bool NT>
 __global__ __launch_bounds__(THREADS) void grad_norm_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(typename T::E), CHUNK = THREADS * V * U;
